@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define LEGO_ABI_VERSION 8
+#define LEGO_ABI_VERSION 9
 #define LEGO_COUNTERS 8
 
 const char* lego_last_error(void);
@@ -407,6 +407,68 @@ int lego_linear_gelu_fwd(const float* x, int ldx, const float* W, int ldw, const
 int lego_linear_bwd_data_gelu(const float* dy, int ldy, const float* W, int ldw, const float* z, int ldz, float* dz, int lddz,
                               int M, int N, int K, void* stream);
 int lego_gelu_bwd(const float* dg, const float* z, float* dz, int64_t n, void* stream);
+
+/* ---- sequence operators: a recurrent encoder of click histories (or any event stream), the norms around its blocks, and the log
+ * probabilities of the next item over a catalogue.  The reference has no counterpart.  Unlike the rest of this header the activations have a
+ * type (`dtype`), rows of any width, and int64 strides in ELEMENTS (channels are contiguous); weights, states and statistics are fp32.
+ * Aligned rows (16 bytes fp32, 8 bytes 16-bit types; widths and strides that are multiples of 4) take vector loads, others one load a
+ * channel.  Masks are bytes, 0 = not there; what a mask hides is never used (it may be NaN).  Workspaces: the sizes come from the
+ * `_workspace` functions below; no call keeps anything in them for the next one. */
+#define LEGO_F32 0
+#define LEGO_BF16 1
+#define LEGO_F16 2
+
+/* Gated linear recurrence, a channel at a time, over x, r, i [n, length, width]:
+ *   a_t = exp(-sharpness softplus(lam) sigmoid(r_t)),   h_t = a_t h_(t-1) + sqrt(1 - a_t^2) sigmoid(i_t) x_t,   h_0 = state (NULL: zeros)
+ * A masked step keeps the state and its row of h is zeros.  h is contiguous; last [n, width] = the state behind the last step.
+ * tiles [n, ceil(length / LEGO_SCAN_TILE), width]: the states that the backward pass starts from; NULL = not wanted.
+ * _bwd: dx, dr, di (contiguous, zeros at masked steps), dlam [width], dstate [n, width] (NULL = not wanted) from gh = d h and glast = d last
+ * (NULL = zeros).  length must be positive, n <= 65535.
+ * _step: one step of n states (mask NULL or [n]): h [n, width] in the activations' type and the new states `next` (may not alias `state`). */
+#define LEGO_SCAN_TILE 64
+int64_t lego_gated_scan_workspace(int n, int length, int width);                 /* floats, for _fwd and for _bwd */
+int lego_gated_scan_fwd(const void* x, int64_t x_sn, int64_t x_sl, const void* r, int64_t r_sn, int64_t r_sl, const void* i, int64_t i_sn,
+                        int64_t i_sl, int dtype, const float* lam, float sharpness, const uint8_t* mask /*nullable*/, int64_t mask_sn,
+                        const float* state /*nullable*/, void* h, float* last, float* tiles /*nullable*/, float* workspace, int64_t workspace_floats,
+                        int n, int length, int width, void* stream);
+int lego_gated_scan_bwd(const void* x, int64_t x_sn, int64_t x_sl, const void* r, int64_t r_sn, int64_t r_sl, const void* i, int64_t i_sn,
+                        int64_t i_sl, const void* gh, int64_t gh_sn, int64_t gh_sl, int dtype, const float* lam, float sharpness,
+                        const uint8_t* mask /*nullable*/, int64_t mask_sn, const float* tiles, const float* glast /*nullable*/, void* dx, void* dr,
+                        void* di, float* dlam, float* dstate /*nullable*/, float* workspace, int64_t workspace_floats, int n, int length, int width,
+                        void* stream);
+int lego_gated_scan_step(const void* x, int64_t x_sn, const void* r, int64_t r_sn, const void* i, int64_t i_sn, int dtype, const float* lam,
+                         float sharpness, const uint8_t* mask /*nullable*/, const float* state, void* h, float* next, int n, int width, void* stream);
+
+/* The norms around a residual block, with its gate and residual scale, one pass over rows of `width` channels:
+ *   y = x + scale act(gate) (o rms(o)^-1 post_w),   next = y rms(y)^-1 next_w,   rms(v) = sqrt(mean(v^2) + eps)
+ * o = NULL: no block (y = x is not written; a plain norm); next_w = NULL: no norm behind it.  act: 0 no gate, 1 sigmoid, 2 silu.
+ * y and next are contiguous; stat [2, rows] keeps 1 / rms(o) and 1 / rms(y) for _bwd (NULL = not wanted).
+ * _bwd: dy (may be NULL where next_w is given) and dn are the gradients of y and next; dx, dout (of o), dgate contiguous; dpost_w, dscale,
+ * dnext_w [width] are written, not added to, in a fixed order of summation. */
+#define LEGO_BLOCK_NORM_MAX_WIDTH 16384
+int64_t lego_block_norm_workspace(int rows, int width);                          /* floats, for _bwd */
+int lego_block_norm_fwd(const void* x, int64_t ldx, const void* o /*nullable*/, int64_t ldo, const void* gate, int64_t ldg, int dtype, int act,
+                        const float* post_w, const float* scale, const float* next_w /*nullable*/, float eps, void* y, void* next,
+                        float* stat /*nullable*/, int rows, int width, void* stream);
+int lego_block_norm_bwd(const void* x, int64_t ldx, const void* o /*nullable*/, int64_t ldo, const void* gate, int64_t ldg, int dtype, int act,
+                        const float* post_w, const float* scale, const float* next_w /*nullable*/, float eps, const void* dy, int64_t lddy,
+                        const void* dn, int64_t lddn, const float* stat, void* dx, void* dout, void* dgate, float* dpost_w, float* dscale,
+                        float* dnext_w, float* workspace, int64_t workspace_floats, int rows, int width, void* stream);
+
+/* Log probabilities of rows of logits [rows, items]: lse, entropy, logp of `targets` (int32, or int64 with targets_64 = 1; outside [0, items)
+ * or NULL: no target, logp 0), and the k <= LEGO_LOGPROBS_MAX_K largest log probabilities with their indices, largest first, equal values by
+ * index.  A row with no item left (all masked or -inf) has lse, logp and top -inf, entropy 0 and indices -1; ranks behind the last item are
+ * (-inf, -1); a row with NaN or +inf has NaN everywhere and indices -1.  mask_ld 0: one mask for all rows.
+ * _bwd: dlogits [rows, items] (contiguous; 0 at masked places and in rows with nothing left) of g_logp, g_entropy [rows] and g_top [rows, k]
+ * (each NULL = zeros), from lse, entropy and index of _fwd. */
+#define LEGO_LOGPROBS_MAX_K 128
+int64_t lego_token_logprobs_workspace(int rows, int items, int dtype, int k);    /* 8-byte words, for _fwd */
+int lego_token_logprobs_fwd(const void* logits, int64_t ld, int dtype, const uint8_t* mask /*nullable*/, int64_t mask_ld, const void* targets,
+                            int targets_64, int k, float* logp, float* entropy, float* lse, float* top, int32_t* index, uint64_t* workspace,
+                            int64_t workspace_words, int rows, int items, void* stream);
+int lego_token_logprobs_bwd(const void* logits, int64_t ld, int dtype, const uint8_t* mask /*nullable*/, int64_t mask_ld, const void* targets,
+                            int targets_64, int k, const float* lse, const float* entropy, const int32_t* index, const float* g_logp,
+                            const float* g_entropy, const float* g_top, void* dlogits, int rows, int items, void* stream);
 
 /* small utilities used by the host side */
 int lego_gather_i32(const int32_t* table, const int32_t* idx, int n_cap, const int32_t* n_dyn, int32_t* out, void* stream);

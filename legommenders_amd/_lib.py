@@ -22,7 +22,7 @@ U64 = ctypes.c_uint64
 U32 = ctypes.c_uint32
 
 
-ABI_VERSION = 8      # == LEGO_ABI_VERSION of include/lego_hip.h this binding was written against
+ABI_VERSION = 9      # == LEGO_ABI_VERSION of include/lego_hip.h this binding was written against
 
 
 class LegoDropout(ctypes.Structure):
@@ -93,12 +93,20 @@ SIGNATURES = {
     "lego_linear_gelu_fwd": [P, I, P, I, P, P, I, P, I, I, I, I, P],
     "lego_linear_bwd_data_gelu": [P, I, P, I, P, I, P, I, I, I, I, P],
     "lego_grouped_metrics": [P, P, P, I, P, I, P, P],
+    "lego_gated_scan_fwd": [P, I64, I64, P, I64, I64, P, I64, I64, I, P, F, P, I64, P, P, P, P, P, I64, I, I, I, P],
+    "lego_gated_scan_bwd": [P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, I, P, F, P, I64, P, P, P, P, P, P, P, P, I64, I, I, I, P],
+    "lego_gated_scan_step": [P, I64, P, I64, P, I64, I, P, F, P, P, P, P, I, I, P],
+    "lego_block_norm_fwd": [P, I64, P, I64, P, I64, I, I, P, P, P, F, P, P, P, I, I, P],
+    "lego_block_norm_bwd": [P, I64, P, I64, P, I64, I, I, P, P, P, F, P, I64, P, I64, P, P, P, P, P, P, P, P, I64, I, I, P],
+    "lego_token_logprobs_fwd": [P, I64, I, P, I64, P, I, I, P, P, P, P, P, P, I64, I, I, P],
+    "lego_token_logprobs_bwd": [P, I64, I, P, I64, P, I, I, P, P, P, P, P, P, P, I, I, P],
 }
 
 
 # entry points that return a VALUE instead of a status (bound separately; tests/test_abi.py checks them against the header too)
 VALUE_FUNCS = {"lego_conv3_wino_du_slabs": [I, I, I], "lego_get_product_mode": []}
-VALUE_FUNCS_I64 = {"lego_sort_rows_temp_bytes": [I]}
+VALUE_FUNCS_I64 = {"lego_sort_rows_temp_bytes": [I], "lego_gated_scan_workspace": [I, I, I], "lego_block_norm_workspace": [I, I],
+                   "lego_token_logprobs_workspace": [I, I, I, I]}
 
 
 class LegoHipError(RuntimeError):

@@ -1,0 +1,341 @@
+// The norms around a residual block, fused with its gate, its residual scale and the next block's norm, and their backward pass
+// (include/lego_hip.h: lego_block_norm_*).  A row of `width` channels:
+//
+//   oh = o (mean o^2 + eps)^-1/2      y = x + scale act(gate) oh post_w      yh = y (mean y^2 + eps)^-1/2      n = yh next_w
+//
+// in one pass: x, o and gate are read once, y and n written once.  Without a block (o = NULL) y = x and only n is written.  HBM-bound: a row
+// lives in the registers of 1, 4 or 16 waves (16- / 8-byte loads, 4 channels a lane), the weights of a lane's channels stay in registers over
+// the rows of a persistent workgroup.
+//
+// Backward, with d = dy + rms_y^-1 (dn next_w - yh mean(dn next_w yh)) the gradient of y:  dx = d,  e = d scale act post_w,
+//   do = rms_o^-1 (e - oh mean(e oh)),  dgate = d scale oh post_w act'(gate),
+//   z = sum_rows d act oh:  dpost_w = z scale, dscale = z post_w;  dnext_w = sum_rows dn yh.
+// y is formed again in fp32 from x, o and gate (the stored y may be rounded to 16 bits); the two root mean squares are kept from the forward
+// pass, so a row needs two sums.  Column sums: registers over a workgroup's rows, LDS over its waves, one partial row a workgroup, and a
+// second launch adds those in a fixed order (no atomics: the same bits every time).
+#include "seq_common.hpp"
+
+namespace lego {
+
+constexpr int BN_BLOCK = 1, BN_NEXT = 2;                               // which of the two halves a call computes
+
+struct Rows { const void* p; int64_t ld; };
+struct BlockNorm {
+    Rows x, o, gate;
+    const float *post_w, *scale, *next_w;
+    float eps;
+    int act, rows, width;
+};
+
+// act(g) and act'(g): 0 none, 1 sigmoid, 2 silu
+__device__ __forceinline__ float gate_act(int act, float g, float& slope) {
+    if (act == 0) { slope = 0.f; return 1.f; }
+    // sigmoid(g) and 1 - sigmoid(g) = sigmoid(-g) from one exponential, the smaller one without a difference
+    const float e = __builtin_amdgcn_exp2f(-1.44269504088896340736f * fabsf(g)), q = __builtin_amdgcn_rcpf(1.f + e), small = e * q;
+    const float s = g < 0.f ? small : q, r = g < 0.f ? q : small;
+    if (act == 1) { slope = s * r; return s; }
+    const float v = g * s;
+    slope = s + v * r;
+    return v;
+}
+
+// sum over the row's waves; `red` is one of two buffers in turn, so that one barrier a sum is enough
+template <int WPR>
+__device__ __forceinline__ float row_sum(float v, float (*red)[16], int& turn) {
+    v = wave_sum(v);
+    if constexpr (WPR > 1) {
+        if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[turn][0];
+#pragma unroll
+        for (int w = 1; w < WPR; ++w) v += red[turn][w];
+        turn ^= 1;
+    }
+    return v;
+}
+
+template <typename T, int MODE, int WPR, int NJ, bool ALIGNED>
+__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_fwd_kernel(BlockNorm p, T* __restrict__ y, T* __restrict__ next, float* __restrict__ stat) {
+    __shared__ float red[2][16];
+    constexpr int RPW = WPR == 1 ? 4 : 1;                              // rows a workgroup holds at a time
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int c0 = 4 * (lane + (WPR == 1 ? 0 : 64 * NJ * wave)), W = p.width;
+    const float inv = 1.f / (float)W;
+    f32x4 wp[NJ], ws[NJ], wn[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const int c = c0 + 256 * j;
+        if constexpr (MODE & BN_BLOCK) { wp[j] = load4<float, ALIGNED>(p.post_w, c, W); ws[j] = load4<float, ALIGNED>(p.scale, c, W); }
+        if constexpr (MODE & BN_NEXT) wn[j] = load4<float, ALIGNED>(p.next_w, c, W);
+    }
+    int turn = 0;
+    for (int64_t row = (int64_t)blockIdx.x * RPW + (WPR == 1 ? wave : 0); row < p.rows; row += (int64_t)gridDim.x * RPW) {
+        f32x4 v[NJ], ov[NJ], gv[NJ];
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int c = c0 + 256 * j;
+            if constexpr (MODE & BN_BLOCK) {
+                ov[j] = load4<T, ALIGNED>((const T*)p.o.p + row * p.o.ld, c, W);
+                if (p.act != 0) gv[j] = load4<T, ALIGNED>((const T*)p.gate.p + row * p.gate.ld, c, W);
+            }
+            v[j] = load4<T, ALIGNED>((const T*)p.x.p + row * p.x.ld, c, W);
+        }
+        if constexpr (MODE & BN_BLOCK) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s += ov[j][k] * ov[j][k];
+            const float ro = rsqrtf(row_sum<WPR>(s, red, turn) * inv + p.eps);
+            if (stat != nullptr && lane == 0 && (WPR == 1 || wave == 0)) stat[row] = ro;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float slope;
+                    const float act = gate_act(p.act, p.act != 0 ? gv[j][k] : 0.f, slope);
+                    v[j][k] += ws[j][k] * act * (ov[j][k] * ro * wp[j][k]);
+                }
+                store4<T, ALIGNED>(y + row * W, c0 + 256 * j, W, v[j]);
+            }
+        }
+        if constexpr (MODE & BN_NEXT) {
+            s = 0.f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s += v[j][k] * v[j][k];
+            const float ry = rsqrtf(row_sum<WPR>(s, red, turn) * inv + p.eps);
+            if (stat != nullptr && lane == 0 && (WPR == 1 || wave == 0)) stat[p.rows + row] = ry;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) store4<T, ALIGNED>(next + row * W, c0 + 256 * j, W, v[j] * ry * wn[j]);
+        }
+    }
+}
+
+template <typename T, int MODE, int WPR, int NJ, bool ALIGNED>
+__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_bwd_kernel(BlockNorm p, Rows dy, Rows dn, const float* __restrict__ stat,
+                                                                               T* __restrict__ dx, T* __restrict__ dout, T* __restrict__ dgate,
+                                                                               float* __restrict__ parts) {
+    __shared__ float red[2][16];
+    constexpr int RPW = WPR == 1 ? 4 : 1;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int c0 = 4 * (lane + (WPR == 1 ? 0 : 64 * NJ * wave)), W = p.width;
+    const float inv = 1.f / (float)W;
+    const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+    f32x4 wp[NJ], ws[NJ], wn[NJ], z[NJ], zn[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const int c = c0 + 256 * j;
+        if constexpr (MODE & BN_BLOCK) { wp[j] = load4<float, ALIGNED>(p.post_w, c, W); ws[j] = load4<float, ALIGNED>(p.scale, c, W); }
+        if constexpr (MODE & BN_NEXT) wn[j] = load4<float, ALIGNED>(p.next_w, c, W);
+        z[j] = zn[j] = zero;
+    }
+    int turn = 0;
+    for (int64_t row = (int64_t)blockIdx.x * RPW + (WPR == 1 ? wave : 0); row < p.rows; row += (int64_t)gridDim.x * RPW) {
+        f32x4 v[NJ], oh[NJ], gv[NJ], d[NJ], t[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int c = c0 + 256 * j;
+            d[j] = dy.p != nullptr ? load4<T, ALIGNED>((const T*)dy.p + row * dy.ld, c, W) : zero;
+            if constexpr (MODE & BN_BLOCK) {
+                oh[j] = load4<T, ALIGNED>((const T*)p.o.p + row * p.o.ld, c, W);
+                gv[j] = p.act != 0 ? load4<T, ALIGNED>((const T*)p.gate.p + row * p.gate.ld, c, W) : zero;
+            }
+            if constexpr (MODE & BN_NEXT) {
+                v[j] = load4<T, ALIGNED>((const T*)p.x.p + row * p.x.ld, c, W);
+                t[j] = load4<T, ALIGNED>((const T*)dn.p + row * dn.ld, c, W);
+            }
+        }
+        if constexpr (MODE & BN_BLOCK) {
+            const float ro = stat[row];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) oh[j] *= ro;
+        }
+        if constexpr (MODE & BN_NEXT) {
+            const float ry = stat[p.rows + row];
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if constexpr (MODE & BN_BLOCK) {
+                        float slope;
+                        v[j][k] += ws[j][k] * gate_act(p.act, gv[j][k], slope) * (oh[j][k] * wp[j][k]);
+                    }
+                    v[j][k] *= ry;                                     // yh
+                    zn[j][k] += t[j][k] * v[j][k];
+                    t[j][k] *= wn[j][k];
+                    s += t[j][k] * v[j][k];
+                }
+            const float m = row_sum<WPR>(s, red, turn) * inv;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) d[j] += ry * (t[j] - v[j] * m);
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) store4<T, ALIGNED>(dx + row * W, c0 + 256 * j, W, d[j]);
+        if constexpr (MODE & BN_BLOCK) {
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                f32x4 dg;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float slope;
+                    const float act = gate_act(p.act, gv[j][k], slope);
+                    z[j][k] += d[j][k] * act * oh[j][k];
+                    const float e = d[j][k] * ws[j][k];
+                    dg[k] = e * oh[j][k] * wp[j][k] * slope;
+                    t[j][k] = e * act * wp[j][k];
+                    s += t[j][k] * oh[j][k];
+                }
+                if (p.act != 0) store4<T, ALIGNED>(dgate + row * W, c0 + 256 * j, W, dg);
+            }
+            const float m = row_sum<WPR>(s, red, turn) * inv, ro = stat[row];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) store4<T, ALIGNED>(dout + row * W, c0 + 256 * j, W, ro * (t[j] - oh[j] * m));
+        }
+    }
+    // this workgroup's partial column sums: parts[workgroup][0] = z, [1] = zn
+    float* mine = parts + (int64_t)blockIdx.x * 2 * W;
+    if constexpr (WPR > 1) {                                           // each wave holds columns of its own
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            if constexpr (MODE & BN_BLOCK) store4<float, ALIGNED>(mine, c0 + 256 * j, W, z[j]);
+            if constexpr (MODE & BN_NEXT) store4<float, ALIGNED>(mine + W, c0 + 256 * j, W, zn[j]);
+        }
+    } else {
+        __shared__ f32x4 fold[4][64 * NJ];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            if (!(MODE & (half == 0 ? BN_BLOCK : BN_NEXT))) continue;
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) fold[wave][lane + 64 * j] = half == 0 ? z[j] : zn[j];
+            __syncthreads();
+            for (int q = threadIdx.x; q < 64 * NJ; q += 256)
+                store4<float, ALIGNED>(mine + half * W, 4 * q, W, (fold[0][q] + fold[1][q]) + (fold[2][q] + fold[3][q]));
+        }
+    }
+}
+
+// the partial rows of all workgroups, 16 columns x 16 row lanes a workgroup
+__global__ __launch_bounds__(256) void block_norm_weights_kernel(const float* __restrict__ parts, int n_parts, int mode, const float* __restrict__ post_w,
+                                                                 const float* __restrict__ scale, float* __restrict__ dpost_w,
+                                                                 float* __restrict__ dscale, float* __restrict__ dnext_w, int width) {
+    __shared__ float red[16][2][17];
+    const int col = threadIdx.x & 15, lane = threadIdx.x >> 4, c = blockIdx.x * 16 + col;
+    float z = 0.f, zn = 0.f;
+    if (c < width)
+        for (int q = lane; q < n_parts; q += 16) {
+            const float* row = parts + (int64_t)q * 2 * width;
+            if (mode & BN_BLOCK) z += row[c];
+            if (mode & BN_NEXT) zn += row[width + c];
+        }
+    red[lane][0][col] = z;
+    red[lane][1][col] = zn;
+    __syncthreads();
+    if (lane == 0 && c < width) {
+#pragma unroll
+        for (int q = 1; q < 16; ++q) { z += red[q][0][col]; zn += red[q][1][col]; }
+        if (mode & BN_BLOCK) { dpost_w[c] = z * scale[c]; dscale[c] = z * post_w[c]; }
+        if (mode & BN_NEXT) dnext_w[c] = zn;
+    }
+}
+
+// waves a row and 4-channel groups a lane: one wave to 1024 channels, then 4 (to 4096), then 16 (to 16384)
+static void block_norm_shape(int width, int& wpr, int& nj) {
+    wpr = width <= 1024 ? 1 : width <= 4096 ? 4 : 16;
+    nj = (width + 256 * wpr - 1) / (256 * wpr);
+}
+
+static int block_norm_grid(int rows, int wpr, int cap) {
+    const int rpw = wpr == 1 ? 4 : 1;
+    const int64_t wgs = ((int64_t)rows + rpw - 1) / rpw;
+    return (int)(wgs < cap ? wgs : cap);
+}
+
+constexpr int BN_FWD_CAP = 2048;
+static int bwd_cap(int wpr) { return wpr == 16 ? 256 : 1024; }
+
+}  // namespace lego
+
+using namespace lego;
+#define ST ((hipStream_t)stream)
+
+// one instantiation for the row's shape; rows that are not aligned take the widest form of their wave count
+#define BY_SHAPE(GO, T, MODE)                                                                                                                      \
+    do {                                                                                                                                           \
+        if (!al) { if (wpr == 1) GO(T, MODE, 1, 4, false); else if (wpr == 4) GO(T, MODE, 4, 4, false); else GO(T, MODE, 16, 4, false); }           \
+        else if (wpr == 1) { if (nj == 1) GO(T, MODE, 1, 1, true); else if (nj == 2) GO(T, MODE, 1, 2, true);                                       \
+                             else if (nj == 3) GO(T, MODE, 1, 3, true); else GO(T, MODE, 1, 4, true); }                                             \
+        else if (wpr == 4) { if (nj == 2) GO(T, MODE, 4, 2, true); else GO(T, MODE, 4, 4, true); }                                                  \
+        else { if (nj == 2) GO(T, MODE, 16, 2, true); else GO(T, MODE, 16, 4, true); }                                                              \
+    } while (0)
+#define BY_MODE(GO, T) do { if (mode == 3) BY_SHAPE(GO, T, 3); else if (mode == BN_BLOCK) BY_SHAPE(GO, T, 1); else BY_SHAPE(GO, T, 2); } while (0)
+
+static int block_norm_check(const char* who, const BlockNorm& p, int dtype, int mode) {
+    LEGO_REQUIRE(dtype == LEGO_F32 || dtype == LEGO_BF16 || dtype == LEGO_F16, "%s: unknown dtype %d", who, dtype);
+    LEGO_REQUIRE(p.rows >= 0 && p.width > 0 && p.width <= LEGO_BLOCK_NORM_MAX_WIDTH, "%s: bad sizes rows=%d, width=%d (1 .. %d)", who, p.rows, p.width,
+                 LEGO_BLOCK_NORM_MAX_WIDTH);
+    LEGO_REQUIRE(mode != 0, "%s: neither a block (o) nor a norm after it (next_w)", who);
+    LEGO_REQUIRE(p.act >= 0 && p.act <= 2, "%s: unknown activation %d of the gate", who, p.act);
+    if (p.rows == 0) return 0;
+    LEGO_REQUIRE(p.x.p != nullptr && (!(mode & BN_BLOCK) || (p.post_w && p.scale && (p.act == 0 || p.gate.p))), "%s: NULL operand", who);
+    return 0;
+}
+
+extern "C" int64_t lego_block_norm_workspace(int rows, int width) {
+    if (rows <= 0 || width <= 0) return 0;
+    int wpr, nj;
+    block_norm_shape(width, wpr, nj);
+    return (int64_t)block_norm_grid(rows, wpr, bwd_cap(wpr)) * 2 * width;
+}
+
+extern "C" int lego_block_norm_fwd(const void* x, int64_t ldx, const void* o, int64_t ldo, const void* gate, int64_t ldg, int dtype, int act,
+                                   const float* post_w, const float* scale, const float* next_w, float eps, void* y, void* next, float* stat, int rows,
+                                   int width, void* stream) {
+    const BlockNorm p{{x, ldx}, {o, ldo}, {gate, ldg}, post_w, scale, next_w, eps, act, rows, width};
+    const int mode = (o != nullptr ? BN_BLOCK : 0) | (next_w != nullptr ? BN_NEXT : 0);
+    if (int rc = block_norm_check("lego_block_norm_fwd", p, dtype, mode)) return rc;
+    if (rows == 0) return 0;
+    LEGO_REQUIRE((!(mode & BN_BLOCK) || y) && (!(mode & BN_NEXT) || next), "lego_block_norm_fwd: NULL output");
+    int wpr, nj;
+    block_norm_shape(width, wpr, nj);
+    const bool al = width % 4 == 0 && (ldx | (o ? ldo : 0) | (act && o ? ldg : 0)) % 4 == 0 && aligned4(x, dtype) && aligned4(o, dtype) && aligned4(gate, dtype) &&
+                    aligned4(y, dtype) && aligned4(next, dtype) && aligned4(post_w, LEGO_F32) && aligned4(scale, LEGO_F32) && aligned4(next_w, LEGO_F32);
+    const dim3 grid(block_norm_grid(rows, wpr, BN_FWD_CAP)), block(wpr == 16 ? 1024 : 256);
+#define GO(T, M, W, J, AL) hipLaunchKernelGGL((block_norm_fwd_kernel<T, M, W, J, AL>), grid, block, 0, ST, p, (T*)y, (T*)next, stat)
+    LEGO_BY_TYPE(dtype, BY_MODE(GO, T));
+#undef GO
+    return check_launch("lego_block_norm_fwd");
+}
+
+extern "C" int lego_block_norm_bwd(const void* x, int64_t ldx, const void* o, int64_t ldo, const void* gate, int64_t ldg, int dtype, int act,
+                                   const float* post_w, const float* scale, const float* next_w, float eps, const void* dy, int64_t lddy,
+                                   const void* dn, int64_t lddn, const float* stat, void* dx, void* dout, void* dgate, float* dpost_w, float* dscale,
+                                   float* dnext_w, float* workspace, int64_t workspace_floats, int rows, int width, void* stream) {
+    const BlockNorm p{{x, ldx}, {o, ldo}, {gate, ldg}, post_w, scale, next_w, eps, act, rows, width};
+    const int mode = (o != nullptr ? BN_BLOCK : 0) | (next_w != nullptr ? BN_NEXT : 0);
+    if (int rc = block_norm_check("lego_block_norm_bwd", p, dtype, mode)) return rc;
+    LEGO_REQUIRE(rows > 0, "lego_block_norm_bwd: no rows: nothing to differentiate");
+    LEGO_REQUIRE(stat && dx && ((mode & BN_NEXT) ? dn && dnext_w : dy != nullptr) && (!(mode & BN_BLOCK) || (dout && dpost_w && dscale && (act == 0 || dgate))),
+                 "lego_block_norm_bwd: NULL operand");
+    LEGO_REQUIRE(workspace != nullptr && workspace_floats >= lego_block_norm_workspace(rows, width),
+                 "lego_block_norm_bwd: workspace of %lld floats, lego_block_norm_workspace says %lld", (long long)workspace_floats,
+                 (long long)lego_block_norm_workspace(rows, width));
+    int wpr, nj;
+    block_norm_shape(width, wpr, nj);
+    const Rows gy{dy, lddy}, gn{dn, lddn};
+    const bool al = width % 4 == 0 && (ldx | (o ? ldo : 0) | (act && o ? ldg : 0) | (dy ? lddy : 0) | (mode & BN_NEXT ? lddn : 0)) % 4 == 0 && aligned4(x, dtype) &&
+                    aligned4(o, dtype) && aligned4(gate, dtype) && aligned4(dy, dtype) && aligned4(dn, dtype) && aligned4(dx, dtype) && aligned4(dout, dtype) &&
+                    aligned4(dgate, dtype) && aligned4(post_w, LEGO_F32) && aligned4(scale, LEGO_F32) && aligned4(next_w, LEGO_F32) && aligned4(workspace, LEGO_F32);
+    const int wgs = block_norm_grid(rows, wpr, bwd_cap(wpr));
+    const dim3 grid(wgs), block(wpr == 16 ? 1024 : 256);
+#define GO(T, M, W, J, AL) hipLaunchKernelGGL((block_norm_bwd_kernel<T, M, W, J, AL>), grid, block, 0, ST, p, gy, gn, stat, (T*)dx, (T*)dout, (T*)dgate, workspace)
+    LEGO_BY_TYPE(dtype, BY_MODE(GO, T));
+#undef GO
+    if (int rc = check_launch("lego_block_norm_bwd")) return rc;
+    hipLaunchKernelGGL(block_norm_weights_kernel, dim3((width + 15) / 16), dim3(256), 0, ST, workspace, wgs, mode, post_w, scale, dpost_w, dscale, dnext_w, width);
+    return check_launch("lego_block_norm_bwd (weights)");
+}

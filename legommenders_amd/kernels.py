@@ -7,6 +7,7 @@ only to own memory / the stream and for index bookkeeping; all arithmetic is in 
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Optional, Tuple
 
@@ -284,3 +285,158 @@ def mhsa_bwd(ctx, gy):
     gx = torch.zeros(n * L, D, dtype=torch.float32, device=dev)
     gx.index_copy_(0, ctx.idx.long(), gxc)
     return gx.view(n, L, D), gin_w, gin_b, gout_w, gout_b
+
+
+# --------------------------------------------------------------------------- sequence operators (recurrence, block norms, log probabilities)
+# These keep the activations' type (fp32 / bf16 / fp16) and take strided rows as they are; the launches go to the tensors' own device.
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+SCAN_TILE = 64              # LEGO_SCAN_TILE
+LOGPROBS_MAX_K = 128        # LEGO_LOGPROBS_MAX_K
+BLOCK_NORM_MAX_WIDTH = 16384
+
+
+def _on(t: torch.Tensor):
+    """the device of `t` as the current one for the launches inside (free where it is already)"""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _last_dense(t: Optional[torch.Tensor]):
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _bytes(mask: Optional[torch.Tensor]):
+    """a mask of any type as bytes, 0 = not there (bool and uint8 as they are)"""
+    if mask is None:
+        return None
+    if mask.dtype not in (torch.bool, torch.uint8):
+        mask = mask != 0
+    return _last_dense(mask.view(torch.uint8) if mask.dtype == torch.bool else mask)
+
+
+def _floats(n, device, dtype=torch.float32):
+    return torch.empty(n, dtype=dtype, device=device) if n else None
+
+
+def gated_scan_fwd(x, r, i, lam, sharpness, mask=None, state=None, keep=False):
+    """-> h [n, length, width], last [n, width] fp32, tiles (the backward pass's states; empty unless `keep`)"""
+    n, length, width = x.shape
+    dev = x.device
+    h = torch.empty(n, length, width, dtype=x.dtype, device=dev)
+    tiles = torch.empty(n, -(-length // SCAN_TILE) if keep else 0, width, dtype=torch.float32, device=dev)
+    if length == 0:
+        return h, torch.zeros(n, width, dtype=torch.float32, device=dev) if state is None else state.clone(memory_format=torch.contiguous_format), tiles
+    last = torch.empty(n, width, dtype=torch.float32, device=dev)
+    x, r, i, mask = _last_dense(x), _last_dense(r), _last_dense(i), _bytes(mask)
+    lam, state = lam.contiguous(), None if state is None else state.contiguous()
+    with _on(x):
+        size = _lib.lib().lego_gated_scan_workspace(n, length, width)
+        ws = _floats(size, dev)
+        call("lego_gated_scan_fwd", _ptr(x), x.stride(0), x.stride(1), _ptr(r), r.stride(0), r.stride(1), _ptr(i), i.stride(0), i.stride(1),
+             _DTYPES[x.dtype], _ptr(lam), sharpness, _ptr(mask), 0 if mask is None else mask.stride(0), _ptr(state), _ptr(h), _ptr(last),
+             _ptr(tiles) if keep else None, _ptr(ws), size, n, length, width, _stream())
+    return h, last, tiles
+
+
+def gated_scan_bwd(gh, glast, x, r, i, lam, sharpness, mask, tiles):
+    """-> dx, dr, di (the activations' type), dlam, dstate (fp32)"""
+    n, length, width = x.shape
+    dx, dr, di = (torch.empty(n, length, width, dtype=x.dtype, device=x.device) for _ in range(3))
+    if n == 0 or length == 0 or width == 0:
+        return dx, dr, di, torch.zeros_like(lam, memory_format=torch.contiguous_format), glast.clone(memory_format=torch.contiguous_format)
+    dlam, dstate = torch.empty(width, dtype=torch.float32, device=x.device), torch.empty(n, width, dtype=torch.float32, device=x.device)
+    x, r, i, gh, mask = _last_dense(x), _last_dense(r), _last_dense(i), _last_dense(gh), _bytes(mask)
+    lam, glast = lam.contiguous(), glast.contiguous()
+    with _on(x):
+        size = _lib.lib().lego_gated_scan_workspace(n, length, width)
+        ws = _floats(size, x.device)
+        call("lego_gated_scan_bwd", _ptr(x), x.stride(0), x.stride(1), _ptr(r), r.stride(0), r.stride(1), _ptr(i), i.stride(0), i.stride(1),
+             _ptr(gh), gh.stride(0), gh.stride(1), _DTYPES[x.dtype], _ptr(lam), sharpness, _ptr(mask), 0 if mask is None else mask.stride(0),
+             _ptr(tiles), _ptr(glast), _ptr(dx), _ptr(dr), _ptr(di), _ptr(dlam), _ptr(dstate), _ptr(ws), size, n, length, width, _stream())
+    return dx, dr, di, dlam, dstate
+
+
+def gated_scan_step(x, r, i, lam, state, sharpness, mask=None):
+    """-> h [n, width] in the activations' type, the new state [n, width] fp32"""
+    n, width = x.shape
+    h, new = torch.empty(n, width, dtype=x.dtype, device=x.device), torch.empty(n, width, dtype=torch.float32, device=x.device)
+    x, r, i, mask = _last_dense(x), _last_dense(r), _last_dense(i), _bytes(mask)
+    lam, state = lam.contiguous(), state.contiguous()
+    mask = None if mask is None else mask.contiguous()
+    with _on(x):
+        call("lego_gated_scan_step", _ptr(x), x.stride(0), _ptr(r), r.stride(0), _ptr(i), i.stride(0), _DTYPES[x.dtype], _ptr(lam), sharpness,
+             _ptr(mask), _ptr(state), _ptr(h), _ptr(new), n, width, _stream())
+    return h, new
+
+
+GATE_ACTS = {None: 0, "sigmoid": 1, "silu": 2}
+
+
+def _ld(t):
+    return 0 if t is None else t.stride(0)
+
+
+def block_norm_fwd(x, o, gate, post_w, scale, next_w, eps, act, keep=False):
+    """2-D rows -> y, next (None where the half is absent), stat [2, rows] (empty unless `keep`)"""
+    rows, width = x.shape
+    dev = x.device
+    y = torch.empty(rows, width, dtype=x.dtype, device=dev) if o is not None else None
+    nxt = torch.empty(rows, width, dtype=x.dtype, device=dev) if next_w is not None else None
+    stat = torch.empty(2, rows if keep else 0, dtype=torch.float32, device=dev)
+    x, o, gate = _last_dense(x), _last_dense(o), _last_dense(gate)
+    post_w, scale, next_w = (None if t is None else t.contiguous() for t in (post_w, scale, next_w))
+    with _on(x):
+        call("lego_block_norm_fwd", _ptr(x), _ld(x), _ptr(o), _ld(o), _ptr(gate), _ld(gate), _DTYPES[x.dtype], act, _ptr(post_w), _ptr(scale),
+             _ptr(next_w), eps, _ptr(y), _ptr(nxt), _ptr(stat) if keep else None, rows, width, _stream())
+    return y, nxt, stat
+
+
+def block_norm_bwd(dy, dn, x, o, gate, post_w, scale, next_w, eps, act, stat):
+    """-> dx, do, dgate (the activations' type), dpost_w, dscale, dnext_w (fp32); None where the operand is absent"""
+    rows, width = x.shape
+    new = lambda t: None if t is None else torch.empty(rows, width, dtype=x.dtype, device=x.device)      # noqa: E731
+    dx, do, dgate = new(x), new(o), new(gate)
+    make = torch.zeros if rows == 0 else torch.empty
+    dpw, dsc, dnw = (None if t is None else make(width, dtype=torch.float32, device=x.device) for t in (post_w, scale, next_w))
+    if rows == 0:
+        return dx, do, dgate, dpw, dsc, dnw
+    x, o, gate, dy, dn = (_last_dense(t) for t in (x, o, gate, dy, dn))
+    post_w, scale, next_w = (None if t is None else t.contiguous() for t in (post_w, scale, next_w))
+    with _on(x):
+        size = _lib.lib().lego_block_norm_workspace(rows, width)
+        ws = _floats(size, x.device)
+        call("lego_block_norm_bwd", _ptr(x), _ld(x), _ptr(o), _ld(o), _ptr(gate), _ld(gate), _DTYPES[x.dtype], act, _ptr(post_w), _ptr(scale),
+             _ptr(next_w), eps, _ptr(dy), _ld(dy), _ptr(dn), _ld(dn), _ptr(stat), _ptr(dx), _ptr(do), _ptr(dgate), _ptr(dpw), _ptr(dsc),
+             _ptr(dnw), _ptr(ws), size, rows, width, _stream())
+    return dx, do, dgate, dpw, dsc, dnw
+
+
+def token_logprobs_fwd(logits, targets, k=0, mask=None):
+    """2-D logits -> logp, entropy, lse [rows], top [rows, k] fp32, index [rows, k] int32"""
+    rows, items = logits.shape
+    f = dict(dtype=torch.float32, device=logits.device)
+    logp, entropy, lse = torch.empty(rows, **f), torch.empty(rows, **f), torch.empty(rows, **f)
+    top, index = torch.empty(rows, k, **f), torch.empty(rows, k, dtype=torch.int32, device=logits.device)
+    logits, mask = _last_dense(logits), _bytes(mask)
+    targets = None if targets is None else targets.contiguous()
+    with _on(logits):
+        size = _lib.lib().lego_token_logprobs_workspace(rows, items, _DTYPES[logits.dtype], k)
+        ws = _floats(size, logits.device, torch.int64)
+        call("lego_token_logprobs_fwd", _ptr(logits), logits.stride(0), _DTYPES[logits.dtype], _ptr(mask), 0 if mask is None else mask.stride(0),
+             _ptr(targets), int(targets is not None and targets.dtype == torch.int64), k, _ptr(logp), _ptr(entropy), _ptr(lse), _ptr(top),
+             _ptr(index), _ptr(ws), size, rows, items, _stream())
+    return logp, entropy, lse, top, index
+
+
+def token_logprobs_bwd(g_logp, g_entropy, g_top, logits, targets, mask, lse, entropy, index):
+    """-> d logits [rows, items], in their type; a gradient that is None counts as zeros"""
+    rows, items = logits.shape
+    out = torch.empty(rows, items, dtype=logits.dtype, device=logits.device)
+    logits, mask = _last_dense(logits), _bytes(mask)
+    targets, g_logp, g_entropy, g_top = (None if t is None else t.contiguous() for t in (targets, g_logp, g_entropy, g_top))
+    if g_top is not None and g_top.numel() == 0:
+        g_top = None
+    with _on(logits):
+        call("lego_token_logprobs_bwd", _ptr(logits), logits.stride(0), _DTYPES[logits.dtype], _ptr(mask), 0 if mask is None else mask.stride(0),
+             _ptr(targets), int(targets is not None and targets.dtype == torch.int64), index.shape[1], _ptr(lse), _ptr(entropy), _ptr(index),
+             _ptr(g_logp), _ptr(g_entropy), _ptr(g_top), _ptr(out), rows, items, _stream())
+    return out
