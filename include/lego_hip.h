@@ -442,7 +442,8 @@ int lego_gated_scan_step(const void* x, int64_t x_sn, const void* r, int64_t r_s
 /* The norms around a residual block, with its gate and residual scale, one pass over rows of `width` channels:
  *   y = x + scale act(gate) (o rms(o)^-1 post_w),   next = y rms(y)^-1 next_w,   rms(v) = sqrt(mean(v^2) + eps)
  * o = NULL: no block (y = x is not written; a plain norm); next_w = NULL: no norm behind it.  act: 0 no gate, 1 sigmoid, 2 silu.
- * y and next are contiguous; stat [2, rows] keeps 1 / rms(o) and 1 / rms(y) for _bwd (NULL = not wanted).
+ * y and next are contiguous; stat [halves, rows] keeps 1 / rms(o) (where there is an o), then 1 / rms(y) (where there is a next_w), for _bwd
+ * (NULL = not wanted).
  * _bwd: dy (may be NULL where next_w is given) and dn are the gradients of y and next; dx, dout (of o), dgate contiguous; dpost_w, dscale,
  * dnext_w [width] are written, not added to, in a fixed order of summation. */
 #define LEGO_BLOCK_NORM_MAX_WIDTH 16384

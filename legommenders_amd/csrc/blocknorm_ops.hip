@@ -106,7 +106,7 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_fwd_kernel(
 #pragma unroll
                 for (int k = 0; k < 4; ++k) s += v[j][k] * v[j][k];
             const float ry = rsqrtf(row_sum<WPR>(s, red, turn) * inv + p.eps);
-            if (stat != nullptr && lane == 0 && (WPR == 1 || wave == 0)) stat[p.rows + row] = ry;
+            if (stat != nullptr && lane == 0 && (WPR == 1 || wave == 0)) stat[(MODE & BN_BLOCK ? p.rows : 0) + row] = ry;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) store4<T, ALIGNED>(next + row * W, c0 + 256 * j, W, v[j] * ry * wn[j]);
         }
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_bwd_kernel(
             for (int j = 0; j < NJ; ++j) oh[j] *= ro;
         }
         if constexpr (MODE & BN_NEXT) {
-            const float ry = stat[p.rows + row];
+            const float ry = stat[(MODE & BN_BLOCK ? p.rows : 0) + row];
             float s = 0.f;
 #pragma unroll
             for (int j = 0; j < NJ; ++j)

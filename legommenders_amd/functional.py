@@ -93,37 +93,42 @@ def dot_ce(user, items):
 
 # ------------------------------------------------------------------------------------------ sequence operators
 # fp32, bf16 or fp16 activations (kept), fp32 weights and states; strided rows are taken as they are.  A step that a mask (0 / False) hides is
-# never used, whatever it holds.
-_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+# never used, whatever it holds.  (The checks run on every call of operators that take microseconds: they build no message unless they refuse.)
+_TYPES = frozenset((torch.float32, torch.bfloat16, torch.float16))
 
 
-def _require(ok, what, why):
-    if not ok:
-        raise LegoHipError(f"{what}: {why}")
+def _refuse(what, why):
+    raise LegoHipError(f"{what}: {why}")
 
 
-def _activations(what, first, **others):
+def _activations(what, first, *others):
     """same shape, type and device for every activation"""
-    _require(isinstance(first, torch.Tensor) and first.dtype in _TYPES, what, "activations are float32, bfloat16 or float16 tensors")
-    for name, t in others.items():
-        _require(isinstance(t, torch.Tensor) and t.shape == first.shape and t.dtype == first.dtype and t.device == first.device, what,
-                 f"{name} has to match the first operand: {tuple(first.shape)}, {first.dtype}, {first.device}")
+    if not isinstance(first, torch.Tensor) or first.dtype not in _TYPES:
+        _refuse(what, "activations are float32, bfloat16 or float16 tensors")
+    for t in others:
+        if not isinstance(t, torch.Tensor) or t.shape != first.shape or t.dtype != first.dtype or t.device != first.device:
+            _refuse(what, f"every activation has to match the first: {tuple(first.shape)}, {first.dtype}, {first.device}")
 
 
-def _weights(what, like, shape, **weights):
-    for name, t in weights.items():
-        _require(isinstance(t, torch.Tensor) and tuple(t.shape) == tuple(shape) and t.dtype == torch.float32 and t.device == like.device, what,
-                 f"{name} has to be float32 of shape {tuple(shape)} on {like.device}")
+def _weights(what, like, shape, *weights):
+    for t in weights:
+        if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != torch.float32 or t.device != like.device:
+            _refuse(what, f"weights and states are float32 tensors on {like.device}, here of shape {tuple(shape)}")
 
 
 def _mask_of(what, mask, shape, like):
-    if mask is not None:
-        _require(isinstance(mask, torch.Tensor) and tuple(mask.shape) == tuple(shape) and mask.device == like.device, what,
-                 f"mask has to be of shape {tuple(shape)} on {like.device}")
+    if not isinstance(mask, torch.Tensor) or mask.shape != shape or mask.device != like.device:
+        _refuse(what, f"mask has to be of shape {tuple(shape)} on {like.device}")
 
 
-def _differentiated(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+def _run(function, op, operands, *rest):
+    """the op on its operands and the rest of its arguments: through its autograd.Function where a gradient is wanted, else below the autograd key"""
+    if torch.is_grad_enabled():
+        for t in operands:
+            if t is not None and t.requires_grad:
+                return function.apply(*rest)
+    with _ops.below_autograd():
+        return op(*rest)
 
 
 def gated_scan(x, r, i, lam, mask=None, state=None, sharpness=8.0):
@@ -132,19 +137,22 @@ def gated_scan(x, r, i, lam, mask=None, state=None, sharpness=8.0):
         a_t = exp(-sharpness softplus(lam) sigmoid(r_t)),   h_t = a_t h_(t-1) + sqrt(1 - a_t^2) sigmoid(i_t) x_t,   h_0 = state (default 0)
 
     -> (h in the activations' type, the state behind the last step [n, width] fp32).  `mask` [n, length]: a masked step keeps the state, its
-    row of h is zeros and its gradients are zeros.  Differentiable in x, r, i, lam and state.  For one more step of many states without a
-    gradient: `gated_scan_step`."""
+    row of h is zeros and its gradients are zeros.  Differentiable (once) in x, r, i, lam and state.  For one more step of many states without a
+    gradient: `gated_scan_step`.  A gate below 2^-126 counts as closed."""
     what = "gated_scan"
-    _activations(what, x, r=r, i=i)
-    _require(x.dim() == 3 and x.shape[0] <= 65535, what, f"x is [n, length, width] with n <= 65535, not {tuple(x.shape)}")
+    _activations(what, x, r, i)
+    if x.dim() != 3 or x.shape[0] > 65535:
+        _refuse(what, f"x is [n, length, width] with n <= 65535, not {tuple(x.shape)}")
     n, length, width = x.shape
-    _weights(what, x, (width,), lam=lam)
+    _weights(what, x, (width,), lam)
     if state is not None:
-        _weights(what, x, (n, width), state=state)
-    _mask_of(what, mask, (n, length), x)
-    _require(sharpness > 0, what, f"sharpness {sharpness} is not positive")
+        _weights(what, x, (n, width), state)
+    if mask is not None:
+        _mask_of(what, mask, (n, length), x)
+    if not sharpness > 0:
+        _refuse(what, f"sharpness {sharpness} is not positive")
     _need_gpu(x, what)
-    h, last, _ = L.gated_scan(x, r, i, lam, mask, state, float(sharpness), _differentiated(x, r, i, lam, state))
+    h, last, _ = _run(_ops.GatedScan, _ops.scan_op, (x, r, i, lam, state), x, r, i, lam, mask, state, float(sharpness), False)
     return h, last
 
 
@@ -152,29 +160,40 @@ def gated_scan_step(x, r, i, lam, state, mask=None, sharpness=8.0):
     """`gated_scan` for one step: x, r, i [n, width], state [n, width] fp32 -> (h [n, width], the new state).  The form that serves: no
     gradient (operands that require one are refused under grad mode), `state` is left as it is.  A masked row keeps its state, its h is zeros."""
     what = "gated_scan_step"
-    _activations(what, x, r=r, i=i)
-    _require(x.dim() == 2, what, f"x is [n, width], not {tuple(x.shape)}")
-    _weights(what, x, (x.shape[1],), lam=lam)
-    _weights(what, x, x.shape, state=state)
-    _mask_of(what, mask, x.shape[:1], x)
-    _require(sharpness > 0, what, f"sharpness {sharpness} is not positive")
-    _require(not _differentiated(x, r, i, lam, state), what, "has no gradient; use gated_scan, or call it under torch.no_grad()")
+    _activations(what, x, r, i)
+    if x.dim() != 2:
+        _refuse(what, f"x is [n, width], not {tuple(x.shape)}")
+    _weights(what, x, x.shape[1:], lam)
+    _weights(what, x, x.shape, state)
+    if mask is not None:
+        _mask_of(what, mask, x.shape[:1], x)
+    if not sharpness > 0:
+        _refuse(what, f"sharpness {sharpness} is not positive")
+    if torch.is_grad_enabled() and (x.requires_grad or r.requires_grad or i.requires_grad or lam.requires_grad or state.requires_grad):
+        _refuse(what, "has no gradient; use gated_scan, or call it under torch.no_grad()")
     _need_gpu(x, what)
-    return L.gated_scan_step(x, r, i, lam, state, mask, float(sharpness))
+    with _ops.below_autograd():
+        return _ops.scan_step_op(x, r, i, lam, state, mask, float(sharpness))
 
 
 def _rows2(t):
-    return None if t is None else t.reshape(-1, t.shape[-1])
+    return t if t is None or t.dim() == 2 else t.reshape(-1, t.shape[-1])
+
+
+def _norm_width(what, x):
+    if x.dim() < 1 or not 0 < x.shape[-1] <= _ops.K.BLOCK_NORM_MAX_WIDTH:
+        _refuse(what, f"the last dimension is 1 to {_ops.K.BLOCK_NORM_MAX_WIDTH} wide, not {tuple(x.shape)}")
 
 
 def rms_norm(x, w, eps=1e-6):
-    """x (mean x^2 + eps)^-1/2 w over the last dimension (at most 16384 wide); x in fp32, bf16 or fp16 (kept), w fp32.  Differentiable."""
+    """x (mean x^2 + eps)^-1/2 w over the last dimension (at most 16384 wide); x in fp32, bf16 or fp16 (kept), w fp32.  Differentiable (once)."""
     what = "rms_norm"
     _activations(what, x)
-    _require(x.dim() >= 1 and 0 < x.shape[-1] <= _ops.K.BLOCK_NORM_MAX_WIDTH, what, f"the last dimension is 1 to {_ops.K.BLOCK_NORM_MAX_WIDTH} wide: {tuple(x.shape)}")
-    _weights(what, x, x.shape[-1:], w=w)
+    _norm_width(what, x)
+    _weights(what, x, x.shape[-1:], w)
     _need_gpu(x, what)
-    return L.block_norm(_rows2(x), None, None, None, None, w, float(eps), 0, _differentiated(x, w))[1].view(x.shape)
+    n = _run(_ops.BlockNorm, _ops.norm_op, (x, w), _rows2(x), None, None, None, None, w, float(eps), 0, False)[1]
+    return n if x.dim() == 2 else n.view(x.shape)
 
 
 def gated_residual_norm(x, o, gate, post_w, scale, next_w=None, eps=1e-6, act="silu"):
@@ -184,16 +203,24 @@ def gated_residual_norm(x, o, gate, post_w, scale, next_w=None, eps=1e-6, act="s
 
     x: the residual stream, o: the block's output, gate: its gate's logits (act "silu" or "sigmoid"; None with act=None: no gate), all of one
     shape [..., width] and type; post_w, scale, next_w [width] fp32.  -> (y, n): n is the norm before the next block (None without next_w),
-    taken from y before its rounding.  Differentiable in every operand."""
+    taken from y before its rounding.  Differentiable (once) in every operand."""
     what = "gated_residual_norm"
-    _require(act in _ops.K.GATE_ACTS and (gate is None) == (act is None), what, f"act {act!r} has to be 'silu' or 'sigmoid' with a gate, None without")
-    _activations(what, x, o=o, **({} if gate is None else {"gate": gate}))
-    _require(x.dim() >= 1 and 0 < x.shape[-1] <= _ops.K.BLOCK_NORM_MAX_WIDTH, what, f"the last dimension is 1 to {_ops.K.BLOCK_NORM_MAX_WIDTH} wide: {tuple(x.shape)}")
-    _weights(what, x, x.shape[-1:], post_w=post_w, scale=scale, **({} if next_w is None else {"next_w": next_w}))
+    if act not in _ops.K.GATE_ACTS or (gate is None) != (act is None):
+        _refuse(what, f"act {act!r} has to be 'silu' or 'sigmoid' with a gate, None without")
+    if gate is None:
+        _activations(what, x, o)
+    else:
+        _activations(what, x, o, gate)
+    _norm_width(what, x)
+    _weights(what, x, x.shape[-1:], post_w, scale)
+    if next_w is not None:
+        _weights(what, x, x.shape[-1:], next_w)
     _need_gpu(x, what)
-    y, n, _ = L.block_norm(_rows2(x), _rows2(o), _rows2(gate), post_w, scale, next_w, float(eps), _ops.K.GATE_ACTS[act],
-                           _differentiated(x, o, gate, post_w, scale, next_w))
-    return y.view(x.shape), None if next_w is None else n.view(x.shape)
+    y, n, _ = _run(_ops.BlockNorm, _ops.norm_op, (x, o, gate, post_w, scale, next_w), _rows2(x), _rows2(o), _rows2(gate), post_w, scale, next_w,
+                   float(eps), _ops.K.GATE_ACTS[act], False)
+    if x.dim() != 2:
+        y, n = y.view(x.shape), n if next_w is None else n.view(x.shape)
+    return y, None if next_w is None else n
 
 
 def token_logprobs(logits, targets=None, k=0, mask=None):
@@ -204,20 +231,29 @@ def token_logprobs(logits, targets=None, k=0, mask=None):
     targets int32 / int64 [...]: an item outside [0, items) -- the pad id -1 -- is no target: logp 0, no gradient.  top is sorted, equal values by
     index; k <= 128.  `mask` [..., items] or [items]: items that are 0 / False there do not exist (the clicks a user has made already).  A row
     with nothing left has logp and top -inf, entropy 0, index -1, and a zero gradient; one with NaN or +inf among its items has NaN.
-    Differentiable in logits through logp, entropy and top; a masked target's logp is -inf."""
+    Differentiable (once) in logits through logp, entropy and top; a masked target's logp is -inf."""
     what = "token_logprobs"
     _activations(what, logits)
-    _require(logits.dim() >= 1 and 0 < logits.shape[-1] <= 1 << 30, what, f"logits are [..., items] with at least one item: {tuple(logits.shape)}")
-    lead, items = logits.shape[:-1], logits.shape[-1]
-    _require(isinstance(k, int) and 0 <= k <= min(_ops.K.LOGPROBS_MAX_K, items), what, f"k = {k} is not 0 to {min(_ops.K.LOGPROBS_MAX_K, items)}")
-    if targets is not None:
-        _require(isinstance(targets, torch.Tensor) and targets.dtype in (torch.int32, torch.int64) and targets.shape == lead
-                 and targets.device == logits.device, what, f"targets are int32 or int64 of shape {tuple(lead)} on {logits.device}")
-    rows = logits.reshape(-1, items)
-    if mask is not None:
-        _require(isinstance(mask, torch.Tensor) and mask.device == logits.device and tuple(mask.shape) in (tuple(logits.shape), (items,)), what,
-                 f"mask has to be of shape {tuple(logits.shape)} or ({items},) on {logits.device}")
-        mask = mask.reshape(-1, items) if mask.dim() > 1 else mask.expand(rows.shape)
+    if logits.dim() < 1 or not 0 < logits.shape[-1] <= 1 << 30:
+        _refuse(what, f"logits are [..., items] with at least one item, not {tuple(logits.shape)}")
+    items = logits.shape[-1]
+    if not isinstance(k, int) or not 0 <= k <= min(_ops.K.LOGPROBS_MAX_K, items):
+        _refuse(what, f"k = {k} is not 0 to {min(_ops.K.LOGPROBS_MAX_K, items)}")
+    if targets is not None and (not isinstance(targets, torch.Tensor) or targets.dtype not in (torch.int32, torch.int64)
+                                or targets.shape != logits.shape[:-1] or targets.device != logits.device):
+        _refuse(what, f"targets are int32 or int64 of shape {tuple(logits.shape[:-1])} on {logits.device}")
+    if mask is not None and (not isinstance(mask, torch.Tensor) or mask.device != logits.device
+                             or (mask.shape != logits.shape and mask.shape != (items,))):
+        _refuse(what, f"mask has to be of shape {tuple(logits.shape)} or ({items},) on {logits.device}")
     _need_gpu(logits, what)
-    logp, entropy, _, top, index = L.token_logprobs(rows, None if targets is None else targets.reshape(-1), mask, k)
+    flat = logits.dim() == 2
+    rows = logits if flat else logits.reshape(-1, items)
+    if mask is not None and mask.dim() != 2:
+        mask = mask.reshape(-1, items) if mask.dim() > 2 else mask.expand(rows.shape)
+    if targets is not None and not flat:
+        targets = targets.reshape(-1)
+    logp, entropy, _, top, index = _run(_ops.TokenLogprobs, _ops.logprobs_op, (logits,), rows, targets, mask, k)
+    if flat:
+        return logp, entropy, top, index
+    lead = logits.shape[:-1]
     return logp.view(lead), entropy.view(lead), top.view(*lead, k), index.view(*lead, k)

@@ -7,7 +7,6 @@ only to own memory / the stream and for index bookkeeping; all arithmetic is in 
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from typing import Optional, Tuple
 
@@ -295,9 +294,17 @@ LOGPROBS_MAX_K = 128        # LEGO_LOGPROBS_MAX_K
 BLOCK_NORM_MAX_WIDTH = 16384
 
 
-def _on(t: torch.Tensor):
-    """the device of `t` as the current one for the launches inside (free where it is already)"""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _launch(t: torch.Tensor, name: str, *args):
+    """the C entry on the device of `t`, and on that device's current stream"""
+    device = t.device.index
+    if device == torch._C._cuda_getDevice():
+        return call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+    with torch.cuda.device(device):
+        return call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
 
 
 def _last_dense(t: Optional[torch.Tensor]):
@@ -317,7 +324,7 @@ def _floats(n, device, dtype=torch.float32):
     return torch.empty(n, dtype=dtype, device=device) if n else None
 
 
-def gated_scan_fwd(x, r, i, lam, sharpness, mask=None, state=None, keep=False):
+def gated_scan_fwd(x, r, i, lam, mask=None, state=None, sharpness=8.0, keep=False):
     """-> h [n, length, width], last [n, width] fp32, tiles (the backward pass's states; empty unless `keep`)"""
     n, length, width = x.shape
     dev = x.device
@@ -328,43 +335,41 @@ def gated_scan_fwd(x, r, i, lam, sharpness, mask=None, state=None, keep=False):
     last = torch.empty(n, width, dtype=torch.float32, device=dev)
     x, r, i, mask = _last_dense(x), _last_dense(r), _last_dense(i), _bytes(mask)
     lam, state = lam.contiguous(), None if state is None else state.contiguous()
-    with _on(x):
-        size = _lib.lib().lego_gated_scan_workspace(n, length, width)
-        ws = _floats(size, dev)
-        call("lego_gated_scan_fwd", _ptr(x), x.stride(0), x.stride(1), _ptr(r), r.stride(0), r.stride(1), _ptr(i), i.stride(0), i.stride(1),
-             _DTYPES[x.dtype], _ptr(lam), sharpness, _ptr(mask), 0 if mask is None else mask.stride(0), _ptr(state), _ptr(h), _ptr(last),
-             _ptr(tiles) if keep else None, _ptr(ws), size, n, length, width, _stream())
+    size = _lib.lib().lego_gated_scan_workspace(n, length, width)
+    ws = _floats(size, dev)
+    _launch(x, "lego_gated_scan_fwd", _at(x), x.stride(0), x.stride(1), _at(r), r.stride(0), r.stride(1), _at(i), i.stride(0), i.stride(1),
+         _DTYPES[x.dtype], _at(lam), sharpness, _at(mask), 0 if mask is None else mask.stride(0), _at(state), _at(h), _at(last),
+         _at(tiles) if keep else None, _at(ws), size, n, length, width)
     return h, last, tiles
 
 
-def gated_scan_bwd(gh, glast, x, r, i, lam, sharpness, mask, tiles):
+def gated_scan_bwd(gh, glast, x, r, i, lam, mask, tiles, sharpness=8.0):
     """-> dx, dr, di (the activations' type), dlam, dstate (fp32)"""
     n, length, width = x.shape
     dx, dr, di = (torch.empty(n, length, width, dtype=x.dtype, device=x.device) for _ in range(3))
     if n == 0 or length == 0 or width == 0:
-        return dx, dr, di, torch.zeros_like(lam, memory_format=torch.contiguous_format), glast.clone(memory_format=torch.contiguous_format)
+        return dx, dr, di, torch.zeros(width, dtype=torch.float32, device=x.device), torch.zeros(n, width, dtype=torch.float32, device=x.device) \
+            if glast is None else glast.clone(memory_format=torch.contiguous_format)
     dlam, dstate = torch.empty(width, dtype=torch.float32, device=x.device), torch.empty(n, width, dtype=torch.float32, device=x.device)
     x, r, i, gh, mask = _last_dense(x), _last_dense(r), _last_dense(i), _last_dense(gh), _bytes(mask)
-    lam, glast = lam.contiguous(), glast.contiguous()
-    with _on(x):
-        size = _lib.lib().lego_gated_scan_workspace(n, length, width)
-        ws = _floats(size, x.device)
-        call("lego_gated_scan_bwd", _ptr(x), x.stride(0), x.stride(1), _ptr(r), r.stride(0), r.stride(1), _ptr(i), i.stride(0), i.stride(1),
-             _ptr(gh), gh.stride(0), gh.stride(1), _DTYPES[x.dtype], _ptr(lam), sharpness, _ptr(mask), 0 if mask is None else mask.stride(0),
-             _ptr(tiles), _ptr(glast), _ptr(dx), _ptr(dr), _ptr(di), _ptr(dlam), _ptr(dstate), _ptr(ws), size, n, length, width, _stream())
+    lam, glast = lam.contiguous(), None if glast is None else glast.contiguous()
+    size = _lib.lib().lego_gated_scan_workspace(n, length, width)
+    ws = _floats(size, x.device)
+    _launch(x, "lego_gated_scan_bwd", _at(x), x.stride(0), x.stride(1), _at(r), r.stride(0), r.stride(1), _at(i), i.stride(0), i.stride(1),
+         _at(gh), gh.stride(0), gh.stride(1), _DTYPES[x.dtype], _at(lam), sharpness, _at(mask), 0 if mask is None else mask.stride(0),
+         _at(tiles), _at(glast), _at(dx), _at(dr), _at(di), _at(dlam), _at(dstate), _at(ws), size, n, length, width)
     return dx, dr, di, dlam, dstate
 
 
-def gated_scan_step(x, r, i, lam, state, sharpness, mask=None):
+def gated_scan_step(x, r, i, lam, state, mask=None, sharpness=8.0):
     """-> h [n, width] in the activations' type, the new state [n, width] fp32"""
     n, width = x.shape
     h, new = torch.empty(n, width, dtype=x.dtype, device=x.device), torch.empty(n, width, dtype=torch.float32, device=x.device)
     x, r, i, mask = _last_dense(x), _last_dense(r), _last_dense(i), _bytes(mask)
     lam, state = lam.contiguous(), state.contiguous()
     mask = None if mask is None else mask.contiguous()
-    with _on(x):
-        call("lego_gated_scan_step", _ptr(x), x.stride(0), _ptr(r), r.stride(0), _ptr(i), i.stride(0), _DTYPES[x.dtype], _ptr(lam), sharpness,
-             _ptr(mask), _ptr(state), _ptr(h), _ptr(new), n, width, _stream())
+    _launch(x, "lego_gated_scan_step", _at(x), x.stride(0), _at(r), r.stride(0), _at(i), i.stride(0), _DTYPES[x.dtype], _at(lam), sharpness,
+         _at(mask), _at(state), _at(h), _at(new), n, width)
     return h, new
 
 
@@ -376,17 +381,16 @@ def _ld(t):
 
 
 def block_norm_fwd(x, o, gate, post_w, scale, next_w, eps, act, keep=False):
-    """2-D rows -> y, next (None where the half is absent), stat [2, rows] (empty unless `keep`)"""
+    """2-D rows -> y, next (None where the half is absent), stat [halves, rows] (no columns unless `keep`)"""
     rows, width = x.shape
     dev = x.device
     y = torch.empty(rows, width, dtype=x.dtype, device=dev) if o is not None else None
     nxt = torch.empty(rows, width, dtype=x.dtype, device=dev) if next_w is not None else None
-    stat = torch.empty(2, rows if keep else 0, dtype=torch.float32, device=dev)
+    stat = torch.empty((o is not None) + (next_w is not None), rows if keep else 0, dtype=torch.float32, device=dev)
     x, o, gate = _last_dense(x), _last_dense(o), _last_dense(gate)
     post_w, scale, next_w = (None if t is None else t.contiguous() for t in (post_w, scale, next_w))
-    with _on(x):
-        call("lego_block_norm_fwd", _ptr(x), _ld(x), _ptr(o), _ld(o), _ptr(gate), _ld(gate), _DTYPES[x.dtype], act, _ptr(post_w), _ptr(scale),
-             _ptr(next_w), eps, _ptr(y), _ptr(nxt), _ptr(stat) if keep else None, rows, width, _stream())
+    _launch(x, "lego_block_norm_fwd", _at(x), _ld(x), _at(o), _ld(o), _at(gate), _ld(gate), _DTYPES[x.dtype], act, _at(post_w), _at(scale),
+         _at(next_w), eps, _at(y), _at(nxt), _at(stat) if keep else None, rows, width)
     return y, nxt, stat
 
 
@@ -401,12 +405,11 @@ def block_norm_bwd(dy, dn, x, o, gate, post_w, scale, next_w, eps, act, stat):
         return dx, do, dgate, dpw, dsc, dnw
     x, o, gate, dy, dn = (_last_dense(t) for t in (x, o, gate, dy, dn))
     post_w, scale, next_w = (None if t is None else t.contiguous() for t in (post_w, scale, next_w))
-    with _on(x):
-        size = _lib.lib().lego_block_norm_workspace(rows, width)
-        ws = _floats(size, x.device)
-        call("lego_block_norm_bwd", _ptr(x), _ld(x), _ptr(o), _ld(o), _ptr(gate), _ld(gate), _DTYPES[x.dtype], act, _ptr(post_w), _ptr(scale),
-             _ptr(next_w), eps, _ptr(dy), _ld(dy), _ptr(dn), _ld(dn), _ptr(stat), _ptr(dx), _ptr(do), _ptr(dgate), _ptr(dpw), _ptr(dsc),
-             _ptr(dnw), _ptr(ws), size, rows, width, _stream())
+    size = _lib.lib().lego_block_norm_workspace(rows, width)
+    ws = _floats(size, x.device)
+    _launch(x, "lego_block_norm_bwd", _at(x), _ld(x), _at(o), _ld(o), _at(gate), _ld(gate), _DTYPES[x.dtype], act, _at(post_w), _at(scale),
+         _at(next_w), eps, _at(dy), _ld(dy), _at(dn), _ld(dn), _at(stat), _at(dx), _at(do), _at(dgate), _at(dpw), _at(dsc),
+         _at(dnw), _at(ws), size, rows, width)
     return dx, do, dgate, dpw, dsc, dnw
 
 
@@ -418,12 +421,11 @@ def token_logprobs_fwd(logits, targets, k=0, mask=None):
     top, index = torch.empty(rows, k, **f), torch.empty(rows, k, dtype=torch.int32, device=logits.device)
     logits, mask = _last_dense(logits), _bytes(mask)
     targets = None if targets is None else targets.contiguous()
-    with _on(logits):
-        size = _lib.lib().lego_token_logprobs_workspace(rows, items, _DTYPES[logits.dtype], k)
-        ws = _floats(size, logits.device, torch.int64)
-        call("lego_token_logprobs_fwd", _ptr(logits), logits.stride(0), _DTYPES[logits.dtype], _ptr(mask), 0 if mask is None else mask.stride(0),
-             _ptr(targets), int(targets is not None and targets.dtype == torch.int64), k, _ptr(logp), _ptr(entropy), _ptr(lse), _ptr(top),
-             _ptr(index), _ptr(ws), size, rows, items, _stream())
+    size = _lib.lib().lego_token_logprobs_workspace(rows, items, _DTYPES[logits.dtype], k)
+    ws = _floats(size, logits.device, torch.int64)
+    _launch(logits, "lego_token_logprobs_fwd", _at(logits), logits.stride(0), _DTYPES[logits.dtype], _at(mask), 0 if mask is None else mask.stride(0),
+         _at(targets), int(targets is not None and targets.dtype == torch.int64), k, _at(logp), _at(entropy), _at(lse), _at(top),
+         _at(index), _at(ws), size, rows, items)
     return logp, entropy, lse, top, index
 
 
@@ -435,8 +437,7 @@ def token_logprobs_bwd(g_logp, g_entropy, g_top, logits, targets, mask, lse, ent
     targets, g_logp, g_entropy, g_top = (None if t is None else t.contiguous() for t in (targets, g_logp, g_entropy, g_top))
     if g_top is not None and g_top.numel() == 0:
         g_top = None
-    with _on(logits):
-        call("lego_token_logprobs_bwd", _ptr(logits), logits.stride(0), _DTYPES[logits.dtype], _ptr(mask), 0 if mask is None else mask.stride(0),
-             _ptr(targets), int(targets is not None and targets.dtype == torch.int64), index.shape[1], _ptr(lse), _ptr(entropy), _ptr(index),
-             _ptr(g_logp), _ptr(g_entropy), _ptr(g_top), _ptr(out), rows, items, _stream())
+    _launch(logits, "lego_token_logprobs_bwd", _at(logits), logits.stride(0), _DTYPES[logits.dtype], _at(mask), 0 if mask is None else mask.stride(0),
+         _at(targets), int(targets is not None and targets.dtype == torch.int64), index.shape[1], _at(lse), _at(entropy), _at(index),
+         _at(g_logp), _at(g_entropy), _at(g_top), _at(out), rows, items)
     return out

@@ -481,164 +481,178 @@ def _(row_user, user_hist, user_hist_len):
 # =============================================================================== sequence operators
 # A recurrent encoder of click histories, the norms around its blocks, next-item log probabilities.  No counterpart in the reference.  They keep
 # the activations' type; an output that a call does not make is an empty tensor (an op's outputs are tensors).
+#
+# Registered through torch.library's definitions themselves, not custom_op: the autograd formula is a plain autograd.Function, which costs the host
+# about half of what custom_op's generic one does (84 against 167 us for a forward and backward pass of three tensors, CPU-bound) -- these
+# operators run for tens of microseconds.  `functional` enters at the Function (a gradient is wanted) or below the autograd key (it is not).
+_LIB = torch.library.Library(NS, "FRAGMENT")
+below_autograd = torch._C._AutoDispatchBelowAutograd
+
+
+def _define(name, schema, impl, fake):
+    _LIB.define(name + schema, tags=(torch.Tag.pt2_compliant_tag,))
+    _LIB.impl(name, impl, "CUDA")
+    register_fake(f"{NS}::{name}", fake, lib=_LIB)
+    return getattr(torch.ops.lego_hip, name).default
+
+
+def _differentiable(name, function, wants):
+    """the Autograd entry of an op: `function` where one of its operands (those at the places `wants`) requires a gradient"""
+    op = getattr(torch.ops.lego_hip, name).default
+
+    def entry(*args):
+        if torch.is_grad_enabled() and any(args[q] is not None and args[q].requires_grad for q in wants):
+            return function.apply(*args)
+        with below_autograd():
+            return op(*args)
+    _LIB.impl(name, entry, "Autograd")
+
+
+def _once(what):
+    if torch.is_grad_enabled():              # create_graph: what these backward passes return has no graph of its own
+        raise RuntimeError(f"{what} is differentiable once (create_graph=True is not supported)")
+
+
 def _or_empty(t, like, dtype=None):
     return like.new_empty(0, dtype=dtype or like.dtype) if t is None else t
 
 
-@_cuda("gated_scan")
-def gated_scan(x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, lam: torch.Tensor, mask: Optional[torch.Tensor], state: Optional[torch.Tensor],
-               sharpness: float, keep: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """h_t = a_t h_(t-1) + sqrt(1 - a_t^2) sigmoid(i_t) x_t with a_t = exp(-sharpness softplus(lam) sigmoid(r_t)) over [n, length, width].
-    Returns (h, the last state [n, width], the tiles' states -- empty unless `keep`: the backward pass starts from them)"""
-    return K.gated_scan_fwd(x.detach(), r.detach(), i.detach(), lam.detach(), sharpness, mask, None if state is None else state.detach(), keep)
-
-
-@register_fake(f"{NS}::gated_scan")
-def _(x, r, i, lam, mask, state, sharpness, keep):
+# ---- gated_scan: h_t = a_t h_(t-1) + sqrt(1 - a_t^2) sigmoid(i_t) x_t, a_t = exp(-sharpness softplus(lam) sigmoid(r_t)), over [n, length, width]
+# -> (h, the last state [n, width], the tiles' states -- empty unless `keep`: the backward pass starts from them)
+def _scan_fake(x, r, i, lam, mask, state, sharpness, keep):
     n, length, width = x.shape
     f = dict(dtype=torch.float32)
     tiles = (length + K.SCAN_TILE - 1) // K.SCAN_TILE if keep else 0
     return x.new_empty(n, length, width), x.new_empty(n, width, **f), x.new_empty(n, tiles, width, **f)
 
 
-@_cuda("gated_scan_bwd")
-def gated_scan_bwd(gh: torch.Tensor, glast: torch.Tensor, x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, lam: torch.Tensor,
-                   mask: Optional[torch.Tensor], tiles: torch.Tensor,
-                   sharpness: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    return K.gated_scan_bwd(gh, glast, x, r, i, lam, sharpness, mask, tiles)
-
-
-@register_fake(f"{NS}::gated_scan_bwd")
-def _(gh, glast, x, r, i, lam, mask, tiles, sharpness):
+def _scan_bwd_fake(gh, glast, x, r, i, lam, mask, tiles, sharpness):
     n, length, width = x.shape
     f = dict(dtype=torch.float32)
     return (x.new_empty(n, length, width), x.new_empty(n, length, width), x.new_empty(n, length, width), x.new_empty(width, **f),
             x.new_empty(n, width, **f))
 
 
-def _scan_setup(ctx, inputs, output):
-    x, r, i, lam, mask, state, sharpness, keep = inputs
-    ctx.save_for_backward(x, r, i, lam, mask, output[2])
-    ctx.args = (sharpness, keep, state is not None)
+scan_op = _define("gated_scan", "(Tensor x, Tensor r, Tensor i, Tensor lam, Tensor? mask, Tensor? state, float sharpness, bool keep) -> (Tensor, Tensor, Tensor)",
+                K.gated_scan_fwd, _scan_fake)
+scan_bwd_op = _define("gated_scan_bwd", "(Tensor gh, Tensor? glast, Tensor x, Tensor r, Tensor i, Tensor lam, Tensor? mask, Tensor tiles, float sharpness)"
+                    " -> (Tensor, Tensor, Tensor, Tensor, Tensor)", K.gated_scan_bwd, _scan_bwd_fake)
+scan_step_op = _define("gated_scan_step", "(Tensor x, Tensor r, Tensor i, Tensor lam, Tensor state, Tensor? mask, float sharpness) -> (Tensor, Tensor)",
+                     K.gated_scan_step, lambda x, r, i, lam, state, mask, sharpness: (x.new_empty(x.shape), x.new_empty(x.shape, dtype=torch.float32)))
 
 
-def _scan_bwd(ctx, gh, glast, gtiles):
-    x, r, i, lam, mask, tiles = ctx.saved_tensors
-    sharpness, keep, has_state = ctx.args
-    if not keep:
-        raise RuntimeError("lego_hip::gated_scan was called with keep=False: its backward pass has no states to start from")
-    dx, dr, di, dlam, dstate = torch.ops.lego_hip.gated_scan_bwd(gh, glast, x, r, i, lam, mask, tiles, sharpness)
-    return dx, dr, di, dlam, None, dstate if has_state else None, None, None
+class GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, r, i, lam, mask, state, sharpness, keep):
+        with below_autograd():
+            h, last, tiles = scan_op(x, r, i, lam, mask, state, sharpness, True)
+        ctx.save_for_backward(x, r, i, lam, mask, tiles)
+        ctx.mark_non_differentiable(tiles)
+        ctx.set_materialize_grads(False)
+        ctx.sharpness, ctx.has_state = sharpness, state is not None
+        return h, last, tiles
+
+    @staticmethod
+    def backward(ctx, gh, glast, gtiles):
+        _once("lego_hip::gated_scan")
+        x, r, i, lam, mask, tiles = ctx.saved_tensors
+        if gh is None:
+            gh = torch.zeros_like(x, memory_format=torch.contiguous_format)
+        dx, dr, di, dlam, dstate = scan_bwd_op(gh, glast, x, r, i, lam, mask, tiles, ctx.sharpness)
+        return dx, dr, di, dlam, None, dstate if ctx.has_state else None, None, None
 
 
-register_autograd(f"{NS}::gated_scan", _scan_bwd, setup_context=_scan_setup)
+_differentiable("gated_scan", GatedScan, (0, 1, 2, 3, 5))
 
 
-@_cuda("gated_scan_step")
-def gated_scan_step(x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, lam: torch.Tensor, state: torch.Tensor, mask: Optional[torch.Tensor],
-                    sharpness: float) -> Tuple[torch.Tensor, torch.Tensor]:
-    """one step of gated_scan for n states (inference): (h [n, width], the new state)"""
-    return K.gated_scan_step(x, r, i, lam, state, sharpness, mask)
-
-
-@register_fake(f"{NS}::gated_scan_step")
-def _(x, r, i, lam, state, mask, sharpness):
-    return x.new_empty(x.shape), x.new_empty(x.shape, dtype=torch.float32)
-
-
-@_cuda("block_norm")
-def block_norm(x: torch.Tensor, o: Optional[torch.Tensor], gate: Optional[torch.Tensor], post_w: Optional[torch.Tensor],
-               scale: Optional[torch.Tensor], next_w: Optional[torch.Tensor], eps: float, act: int,
-               keep: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """y = x + scale act(gate) rmsnorm(o) post_w;  next = rmsnorm(y) next_w, over rows [rows, width].  Returns (y, next, the rows'
-    1 / root mean squares [2, rows]); y is empty without o, next without next_w, the last unless `keep`"""
-    d = lambda t: None if t is None else t.detach()      # noqa: E731
-    y, nxt, stat = K.block_norm_fwd(d(x), d(o), d(gate), d(post_w), d(scale), d(next_w), eps, act, keep)
+# ---- block_norm: y = x + scale act(gate) rmsnorm(o) post_w, next = rmsnorm(y) next_w, over rows [rows, width] -> (y, next, the rows'
+# 1 / root mean squares [halves, rows]); y is empty without o, next without next_w, the last unless `keep`
+def _norm_impl(x, o, gate, post_w, scale, next_w, eps, act, keep):
+    y, nxt, stat = K.block_norm_fwd(x, o, gate, post_w, scale, next_w, eps, act, keep)
     return _or_empty(y, x), _or_empty(nxt, x), stat
 
 
-@register_fake(f"{NS}::block_norm")
-def _(x, o, gate, post_w, scale, next_w, eps, act, keep):
+def _norm_fake(x, o, gate, post_w, scale, next_w, eps, act, keep):
     rows, width = x.shape
     return (x.new_empty(0) if o is None else x.new_empty(rows, width), x.new_empty(0) if next_w is None else x.new_empty(rows, width),
-            x.new_empty(2, rows if keep else 0, dtype=torch.float32))
+            x.new_empty((o is not None) + (next_w is not None), rows if keep else 0, dtype=torch.float32))
 
 
-@_cuda("block_norm_bwd")
-def block_norm_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], x: torch.Tensor, o: Optional[torch.Tensor], gate: Optional[torch.Tensor],
-                   post_w: Optional[torch.Tensor], scale: Optional[torch.Tensor], next_w: Optional[torch.Tensor], stat: torch.Tensor, eps: float,
-                   act: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+def _norm_bwd_impl(dy, dn, x, o, gate, post_w, scale, next_w, stat, eps, act):
     out = K.block_norm_bwd(dy, dn, x, o, gate, post_w, scale, next_w, eps, act, stat)
     return tuple(_or_empty(t, x, torch.float32 if q >= 3 else None) for q, t in enumerate(out))
 
 
-@register_fake(f"{NS}::block_norm_bwd")
-def _(dy, dn, x, o, gate, post_w, scale, next_w, stat, eps, act):
+def _norm_bwd_fake(dy, dn, x, o, gate, post_w, scale, next_w, stat, eps, act):
     rows = [x.new_empty(0) if t is None else x.new_empty(x.shape) for t in (x, o, gate)]
-    weights = [x.new_empty(0 if t is None else x.shape[1], dtype=torch.float32) for t in (post_w, scale, next_w)]
-    return tuple(rows + weights)
+    return tuple(rows + [x.new_empty(0 if t is None else x.shape[1], dtype=torch.float32) for t in (post_w, scale, next_w)])
 
 
-def _norm_setup(ctx, inputs, output):
-    x, o, gate, post_w, scale, next_w, eps, act, keep = inputs
-    ctx.save_for_backward(x, o, gate, post_w, scale, next_w, output[2])
-    ctx.args = (eps, act, keep)
+norm_op = _define("block_norm", "(Tensor x, Tensor? o, Tensor? gate, Tensor? post_w, Tensor? scale, Tensor? next_w, float eps, int act, bool keep)"
+                " -> (Tensor, Tensor, Tensor)", _norm_impl, _norm_fake)
+norm_bwd_op = _define("block_norm_bwd", "(Tensor? dy, Tensor? dn, Tensor x, Tensor? o, Tensor? gate, Tensor? post_w, Tensor? scale, Tensor? next_w, Tensor stat,"
+                    " float eps, int act) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)", _norm_bwd_impl, _norm_bwd_fake)
 
 
-def _norm_bwd(ctx, gy, gn, gstat):
-    x, o, gate, post_w, scale, next_w, stat = ctx.saved_tensors
-    eps, act, keep = ctx.args
-    if not keep:
-        raise RuntimeError("lego_hip::block_norm was called with keep=False: its backward pass has no statistics")
-    out = torch.ops.lego_hip.block_norm_bwd(gy if o is not None else None, gn if next_w is not None else None, x, o, gate, post_w, scale, next_w,
-                                            stat, eps, act)
-    return tuple(g if t is not None else None for g, t in zip(out, (x, o, gate, post_w, scale, next_w))) + (None, None, None)
+class BlockNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, o, gate, post_w, scale, next_w, eps, act, keep):
+        with below_autograd():
+            y, nxt, stat = norm_op(x, o, gate, post_w, scale, next_w, eps, act, True)
+        ctx.save_for_backward(x, o, gate, post_w, scale, next_w, stat)
+        ctx.mark_non_differentiable(*(t for t in (y, nxt, stat) if t is stat or t.numel() == 0 and x.numel() > 0))
+        ctx.set_materialize_grads(False)
+        ctx.eps, ctx.act = eps, act
+        return y, nxt, stat
+
+    @staticmethod
+    def backward(ctx, gy, gn, gstat):
+        _once("lego_hip::block_norm")
+        x, o, gate, post_w, scale, next_w, stat = ctx.saved_tensors
+        if next_w is not None and gn is None:
+            gn = torch.zeros_like(x, memory_format=torch.contiguous_format)
+        if next_w is None and gy is None:
+            gy = torch.zeros_like(x, memory_format=torch.contiguous_format)
+        out = norm_bwd_op(gy if o is not None else None, gn if next_w is not None else None, x, o, gate, post_w, scale, next_w, stat, ctx.eps, ctx.act)
+        return tuple(None if t is None else g for g, t in zip(out, (x, o, gate, post_w, scale, next_w))) + (None, None, None)
 
 
-register_autograd(f"{NS}::block_norm", _norm_bwd, setup_context=_norm_setup)
+_differentiable("block_norm", BlockNorm, range(6))
 
 
-@_cuda("token_logprobs")
-def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor], mask: Optional[torch.Tensor],
-                   k: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """rows of logits [rows, items] -> (log probability of the target, entropy, log-sum-exp, the k largest log probabilities, their indices)"""
-    return K.token_logprobs_fwd(logits.detach(), targets, k, mask)
-
-
-@register_fake(f"{NS}::token_logprobs")
-def _(logits, targets, mask, k):
+# ---- token_logprobs: rows of logits [rows, items] -> (log probability of the target, entropy, log-sum-exp, the k largest log probabilities, their
+# indices)
+def _lp_fake(logits, targets, mask, k):
     rows, f = logits.shape[0], dict(dtype=torch.float32)
     return (logits.new_empty(rows, **f), logits.new_empty(rows, **f), logits.new_empty(rows, **f), logits.new_empty(rows, k, **f),
             logits.new_empty(rows, k, dtype=torch.int32))
 
 
-@_cuda("token_logprobs_bwd")
-def token_logprobs_bwd(g_logp: Optional[torch.Tensor], g_entropy: Optional[torch.Tensor], g_top: Optional[torch.Tensor], logits: torch.Tensor,
-                       targets: Optional[torch.Tensor], mask: Optional[torch.Tensor], lse: torch.Tensor, entropy: torch.Tensor,
-                       index: torch.Tensor) -> torch.Tensor:
-    return K.token_logprobs_bwd(g_logp, g_entropy, g_top, logits, targets, mask, lse, entropy, index)
+logprobs_op = _define("token_logprobs", "(Tensor logits, Tensor? targets, Tensor? mask, SymInt k) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
+              lambda logits, targets, mask, k: K.token_logprobs_fwd(logits, targets, k, mask), _lp_fake)
+logprobs_bwd_op = _define("token_logprobs_bwd", "(Tensor? g_logp, Tensor? g_entropy, Tensor? g_top, Tensor logits, Tensor? targets, Tensor? mask, Tensor lse,"
+                  " Tensor entropy, Tensor index) -> Tensor", K.token_logprobs_bwd,
+                  lambda g_logp, g_entropy, g_top, logits, targets, mask, lse, entropy, index: logits.new_empty(logits.shape))
 
 
-@register_fake(f"{NS}::token_logprobs_bwd")
-def _(g_logp, g_entropy, g_top, logits, targets, mask, lse, entropy, index):
-    return logits.new_empty(logits.shape)
+class TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, mask, k):
+        with below_autograd():
+            logp, entropy, lse, top, index = logprobs_op(logits, targets, mask, k)
+        ctx.save_for_backward(logits, targets, mask, lse, entropy, index)
+        ctx.mark_non_differentiable(lse, index)
+        ctx.set_materialize_grads(False)
+        return logp, entropy, lse, top, index
+
+    @staticmethod
+    def backward(ctx, g_logp, g_entropy, g_lse, g_top, g_index):
+        _once("lego_hip::token_logprobs")
+        logits, targets, mask, lse, entropy, index = ctx.saved_tensors
+        return logprobs_bwd_op(g_logp, g_entropy, g_top, logits, targets, mask, lse, entropy, index), None, None, None
 
 
-def _lp_setup(ctx, inputs, output):
-    logits, targets, mask, k = inputs
-    ctx.save_for_backward(logits, targets, mask, output[1], output[2], output[4])
-    ctx.mark_non_differentiable(output[2], output[4])
-    ctx.set_materialize_grads(False)
-
-
-def _lp_bwd(ctx, g_logp, g_entropy, g_lse, g_top, g_index):
-    logits, targets, mask, entropy, lse, index = ctx.saved_tensors
-    if g_logp is None and g_entropy is None and g_top is None:
-        return None, None, None, None
-    return torch.ops.lego_hip.token_logprobs_bwd(g_logp, g_entropy, g_top, logits, targets, mask, lse, entropy, index), None, None, None
-
-
-register_autograd(f"{NS}::token_logprobs", _lp_bwd, setup_context=_lp_setup)
+_differentiable("token_logprobs", TokenLogprobs, (0,))
 
 
 OPS = ("gather_rows", "scatter_add_rows", "linear", "linear_bwd", "glove_project", "glove_project_bwd", "glove_project_bwd_table", "conv3_relu_mask",
