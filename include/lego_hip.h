@@ -411,8 +411,7 @@ int lego_gelu_bwd(const float* dg, const float* z, float* dz, int64_t n, void* s
 /* ---- sequence operators: a recurrent encoder of click histories (or any event stream), the norms around its blocks, and the log
  * probabilities of the next item over a catalogue.  The reference has no counterpart.  Unlike the rest of this header the activations have a
  * type (`dtype`), rows of any width, and int64 strides in ELEMENTS (channels are contiguous); weights, states and statistics are fp32.
- * Aligned rows (16 bytes fp32, 8 bytes 16-bit types; widths and strides that are multiples of 4) take vector loads, others one load a
- * channel.  Masks are bytes, 0 = not there; what a mask hides is never used (it may be NaN).  Workspaces: the sizes come from the
+ * Rows need no alignment beyond their elements'.  Masks are bytes, 0 = not there; what a mask hides is never used (it may be NaN).  Workspaces: the sizes come from the
  * `_workspace` functions below; no call keeps anything in them for the next one. */
 #define LEGO_F32 0
 #define LEGO_BF16 1

@@ -54,7 +54,7 @@ __device__ __forceinline__ float row_sum(float v, float (*red)[16], int& turn) {
     return v;
 }
 
-template <typename T, int MODE, int WPR, int NJ, bool ALIGNED>
+template <typename T, int MODE, int WPR, int NJ, bool FULL>
 __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_fwd_kernel(BlockNorm p, T* __restrict__ y, T* __restrict__ next, float* __restrict__ stat) {
     __shared__ float red[2][16];
     constexpr int RPW = WPR == 1 ? 4 : 1;                              // rows a workgroup holds at a time
@@ -65,8 +65,8 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_fwd_kernel(
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
         const int c = c0 + 256 * j;
-        if constexpr (MODE & BN_BLOCK) { wp[j] = load4<float, ALIGNED>(p.post_w, c, W); ws[j] = load4<float, ALIGNED>(p.scale, c, W); }
-        if constexpr (MODE & BN_NEXT) wn[j] = load4<float, ALIGNED>(p.next_w, c, W);
+        if constexpr (MODE & BN_BLOCK) { wp[j] = load<float, 4, FULL>(p.post_w, c, W); ws[j] = load<float, 4, FULL>(p.scale, c, W); }
+        if constexpr (MODE & BN_NEXT) wn[j] = load<float, 4, FULL>(p.next_w, c, W);
     }
     int turn = 0;
     for (int64_t row = (int64_t)blockIdx.x * RPW + (WPR == 1 ? wave : 0); row < p.rows; row += (int64_t)gridDim.x * RPW) {
@@ -76,10 +76,10 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_fwd_kernel(
         for (int j = 0; j < NJ; ++j) {
             const int c = c0 + 256 * j;
             if constexpr (MODE & BN_BLOCK) {
-                ov[j] = load4<T, ALIGNED>((const T*)p.o.p + row * p.o.ld, c, W);
-                if (p.act != 0) gv[j] = load4<T, ALIGNED>((const T*)p.gate.p + row * p.gate.ld, c, W);
+                ov[j] = load<T, 4, FULL>((const T*)p.o.p + row * p.o.ld, c, W);
+                if (p.act != 0) gv[j] = load<T, 4, FULL>((const T*)p.gate.p + row * p.gate.ld, c, W);
             }
-            v[j] = load4<T, ALIGNED>((const T*)p.x.p + row * p.x.ld, c, W);
+            v[j] = load<T, 4, FULL>((const T*)p.x.p + row * p.x.ld, c, W);
         }
         if constexpr (MODE & BN_BLOCK) {
 #pragma unroll
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_fwd_kernel(
                     const float act = gate_act(p.act, p.act != 0 ? gv[j][k] : 0.f, slope);
                     v[j][k] += ws[j][k] * act * (ov[j][k] * ro * wp[j][k]);
                 }
-                store4<T, ALIGNED>(y + row * W, c0 + 256 * j, W, v[j]);
+                store<T, 4, FULL>(y + row * W, c0 + 256 * j, W, v[j]);
             }
         }
         if constexpr (MODE & BN_NEXT) {
@@ -108,12 +108,12 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_fwd_kernel(
             const float ry = rsqrtf(row_sum<WPR>(s, red, turn) * inv + p.eps);
             if (stat != nullptr && lane == 0 && (WPR == 1 || wave == 0)) stat[(MODE & BN_BLOCK ? p.rows : 0) + row] = ry;
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) store4<T, ALIGNED>(next + row * W, c0 + 256 * j, W, v[j] * ry * wn[j]);
+            for (int j = 0; j < NJ; ++j) store<T, 4, FULL>(next + row * W, c0 + 256 * j, W, v[j] * ry * wn[j]);
         }
     }
 }
 
-template <typename T, int MODE, int WPR, int NJ, bool ALIGNED>
+template <typename T, int MODE, int WPR, int NJ, bool FULL>
 __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_bwd_kernel(BlockNorm p, Rows dy, Rows dn, const float* __restrict__ stat,
                                                                                T* __restrict__ dx, T* __restrict__ dout, T* __restrict__ dgate,
                                                                                float* __restrict__ parts) {
@@ -127,8 +127,8 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_bwd_kernel(
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
         const int c = c0 + 256 * j;
-        if constexpr (MODE & BN_BLOCK) { wp[j] = load4<float, ALIGNED>(p.post_w, c, W); ws[j] = load4<float, ALIGNED>(p.scale, c, W); }
-        if constexpr (MODE & BN_NEXT) wn[j] = load4<float, ALIGNED>(p.next_w, c, W);
+        if constexpr (MODE & BN_BLOCK) { wp[j] = load<float, 4, FULL>(p.post_w, c, W); ws[j] = load<float, 4, FULL>(p.scale, c, W); }
+        if constexpr (MODE & BN_NEXT) wn[j] = load<float, 4, FULL>(p.next_w, c, W);
         z[j] = zn[j] = zero;
     }
     int turn = 0;
@@ -137,14 +137,14 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_bwd_kernel(
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const int c = c0 + 256 * j;
-            d[j] = dy.p != nullptr ? load4<T, ALIGNED>((const T*)dy.p + row * dy.ld, c, W) : zero;
+            d[j] = dy.p != nullptr ? load<T, 4, FULL>((const T*)dy.p + row * dy.ld, c, W) : zero;
             if constexpr (MODE & BN_BLOCK) {
-                oh[j] = load4<T, ALIGNED>((const T*)p.o.p + row * p.o.ld, c, W);
-                gv[j] = p.act != 0 ? load4<T, ALIGNED>((const T*)p.gate.p + row * p.gate.ld, c, W) : zero;
+                oh[j] = load<T, 4, FULL>((const T*)p.o.p + row * p.o.ld, c, W);
+                gv[j] = p.act != 0 ? load<T, 4, FULL>((const T*)p.gate.p + row * p.gate.ld, c, W) : zero;
             }
             if constexpr (MODE & BN_NEXT) {
-                v[j] = load4<T, ALIGNED>((const T*)p.x.p + row * p.x.ld, c, W);
-                t[j] = load4<T, ALIGNED>((const T*)dn.p + row * dn.ld, c, W);
+                v[j] = load<T, 4, FULL>((const T*)p.x.p + row * p.x.ld, c, W);
+                t[j] = load<T, 4, FULL>((const T*)dn.p + row * dn.ld, c, W);
             }
         }
         if constexpr (MODE & BN_BLOCK) {
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_bwd_kernel(
             for (int j = 0; j < NJ; ++j) d[j] += ry * (t[j] - v[j] * m);
         }
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) store4<T, ALIGNED>(dx + row * W, c0 + 256 * j, W, d[j]);
+        for (int j = 0; j < NJ; ++j) store<T, 4, FULL>(dx + row * W, c0 + 256 * j, W, d[j]);
         if constexpr (MODE & BN_BLOCK) {
             float s = 0.f;
 #pragma unroll
@@ -189,11 +189,11 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_bwd_kernel(
                     t[j][k] = e * act * wp[j][k];
                     s += t[j][k] * oh[j][k];
                 }
-                if (p.act != 0) store4<T, ALIGNED>(dgate + row * W, c0 + 256 * j, W, dg);
+                if (p.act != 0) store<T, 4, FULL>(dgate + row * W, c0 + 256 * j, W, dg);
             }
             const float m = row_sum<WPR>(s, red, turn) * inv, ro = stat[row];
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) store4<T, ALIGNED>(dout + row * W, c0 + 256 * j, W, ro * (t[j] - oh[j] * m));
+            for (int j = 0; j < NJ; ++j) store<T, 4, FULL>(dout + row * W, c0 + 256 * j, W, ro * (t[j] - oh[j] * m));
         }
     }
     // this workgroup's partial column sums: parts[workgroup][0] = z, [1] = zn
@@ -201,8 +201,8 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_bwd_kernel(
     if constexpr (WPR > 1) {                                           // each wave holds columns of its own
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            if constexpr (MODE & BN_BLOCK) store4<float, ALIGNED>(mine, c0 + 256 * j, W, z[j]);
-            if constexpr (MODE & BN_NEXT) store4<float, ALIGNED>(mine + W, c0 + 256 * j, W, zn[j]);
+            if constexpr (MODE & BN_BLOCK) store<float, 4, FULL>(mine, c0 + 256 * j, W, z[j]);
+            if constexpr (MODE & BN_NEXT) store<float, 4, FULL>(mine + W, c0 + 256 * j, W, zn[j]);
         }
     } else {
         __shared__ f32x4 fold[4][64 * NJ];
@@ -214,32 +214,40 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_bwd_kernel(
             for (int j = 0; j < NJ; ++j) fold[wave][lane + 64 * j] = half == 0 ? z[j] : zn[j];
             __syncthreads();
             for (int q = threadIdx.x; q < 64 * NJ; q += 256)
-                store4<float, ALIGNED>(mine + half * W, 4 * q, W, (fold[0][q] + fold[1][q]) + (fold[2][q] + fold[3][q]));
+                store<float, 4, FULL>(mine + half * W, 4 * q, W, (fold[0][q] + fold[1][q]) + (fold[2][q] + fold[3][q]));
         }
     }
 }
 
-// the partial rows of all workgroups, 16 columns x 16 row lanes a workgroup
-__global__ __launch_bounds__(256) void block_norm_weights_kernel(const float* __restrict__ parts, int n_parts, int mode, const float* __restrict__ post_w,
-                                                                 const float* __restrict__ scale, float* __restrict__ dpost_w,
-                                                                 float* __restrict__ dscale, float* __restrict__ dnext_w, int width) {
-    __shared__ float red[16][2][17];
+// the partial rows of all workgroups: 16 columns x 64 row lanes a workgroup, 8 rows of a lane in flight
+__global__ __launch_bounds__(1024) void block_norm_weights_kernel(const float* __restrict__ parts, int n_parts, int mode, const float* __restrict__ post_w,
+                                                                  const float* __restrict__ scale, float* __restrict__ dpost_w,
+                                                                  float* __restrict__ dscale, float* __restrict__ dnext_w, int width) {
+    __shared__ float red[2][64][17];
     const int col = threadIdx.x & 15, lane = threadIdx.x >> 4, c = blockIdx.x * 16 + col;
-    float z = 0.f, zn = 0.f;
-    if (c < width)
-        for (int q = lane; q < n_parts; q += 16) {
-            const float* row = parts + (int64_t)q * 2 * width;
-            if (mode & BN_BLOCK) z += row[c];
-            if (mode & BN_NEXT) zn += row[width + c];
-        }
-    red[lane][0][col] = z;
-    red[lane][1][col] = zn;
-    __syncthreads();
-    if (lane == 0 && c < width) {
 #pragma unroll
-        for (int q = 1; q < 16; ++q) { z += red[q][0][col]; zn += red[q][1][col]; }
-        if (mode & BN_BLOCK) { dpost_w[c] = z * scale[c]; dscale[c] = z * post_w[c]; }
-        if (mode & BN_NEXT) dnext_w[c] = zn;
+    for (int half = 0; half < 2; ++half) {
+        if (!(mode & (half == 0 ? BN_BLOCK : BN_NEXT))) continue;
+        float s = 0.f;
+        if (c < width)
+            for (int q = lane; q < n_parts; q += 64 * 8) {
+                float v[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) v[u] = q + 64 * u < n_parts ? parts[((int64_t)(q + 64 * u) * 2 + half) * width + c] : 0.f;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) s += v[u];
+            }
+        red[half][lane][col] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32 && c < width) {
+        const int half = threadIdx.x >> 4;
+        if (mode & (half == 0 ? BN_BLOCK : BN_NEXT)) {
+            float s = 0.f;
+            for (int q = 0; q < 64; ++q) s += red[half][q][col];
+            if (half == 0) { dpost_w[c] = s * scale[c]; dscale[c] = s * post_w[c]; }
+            else dnext_w[c] = s;
+        }
     }
 }
 
@@ -263,10 +271,10 @@ static int bwd_cap(int wpr) { return wpr == 16 ? 256 : 1024; }
 using namespace lego;
 #define ST ((hipStream_t)stream)
 
-// one instantiation for the row's shape; rows that are not aligned take the widest form of their wave count
+// one instantiation for the row's shape; widths that are no multiple of 4 take the widest form of their wave count
 #define BY_SHAPE(GO, T, MODE)                                                                                                                      \
     do {                                                                                                                                           \
-        if (!al) { if (wpr == 1) GO(T, MODE, 1, 4, false); else if (wpr == 4) GO(T, MODE, 4, 4, false); else GO(T, MODE, 16, 4, false); }           \
+        if (!full) { if (wpr == 1) GO(T, MODE, 1, 4, false); else if (wpr == 4) GO(T, MODE, 4, 4, false); else GO(T, MODE, 16, 4, false); }           \
         else if (wpr == 1) { if (nj == 1) GO(T, MODE, 1, 1, true); else if (nj == 2) GO(T, MODE, 1, 2, true);                                       \
                              else if (nj == 3) GO(T, MODE, 1, 3, true); else GO(T, MODE, 1, 4, true); }                                             \
         else if (wpr == 4) { if (nj == 2) GO(T, MODE, 4, 2, true); else GO(T, MODE, 4, 4, true); }                                                  \
@@ -302,10 +310,9 @@ extern "C" int lego_block_norm_fwd(const void* x, int64_t ldx, const void* o, in
     LEGO_REQUIRE((!(mode & BN_BLOCK) || y) && (!(mode & BN_NEXT) || next), "lego_block_norm_fwd: NULL output");
     int wpr, nj;
     block_norm_shape(width, wpr, nj);
-    const bool al = width % 4 == 0 && (ldx | (o ? ldo : 0) | (act && o ? ldg : 0)) % 4 == 0 && aligned4(x, dtype) && aligned4(o, dtype) && aligned4(gate, dtype) &&
-                    aligned4(y, dtype) && aligned4(next, dtype) && aligned4(post_w, LEGO_F32) && aligned4(scale, LEGO_F32) && aligned4(next_w, LEGO_F32);
+    const bool full = width % 4 == 0;
     const dim3 grid(block_norm_grid(rows, wpr, BN_FWD_CAP)), block(wpr == 16 ? 1024 : 256);
-#define GO(T, M, W, J, AL) hipLaunchKernelGGL((block_norm_fwd_kernel<T, M, W, J, AL>), grid, block, 0, ST, p, (T*)y, (T*)next, stat)
+#define GO(T, M, W, J, F) hipLaunchKernelGGL((block_norm_fwd_kernel<T, M, W, J, F>), grid, block, 0, ST, p, (T*)y, (T*)next, stat)
     LEGO_BY_TYPE(dtype, BY_MODE(GO, T));
 #undef GO
     return check_launch("lego_block_norm_fwd");
@@ -327,15 +334,13 @@ extern "C" int lego_block_norm_bwd(const void* x, int64_t ldx, const void* o, in
     int wpr, nj;
     block_norm_shape(width, wpr, nj);
     const Rows gy{dy, lddy}, gn{dn, lddn};
-    const bool al = width % 4 == 0 && (ldx | (o ? ldo : 0) | (act && o ? ldg : 0) | (dy ? lddy : 0) | (mode & BN_NEXT ? lddn : 0)) % 4 == 0 && aligned4(x, dtype) &&
-                    aligned4(o, dtype) && aligned4(gate, dtype) && aligned4(dy, dtype) && aligned4(dn, dtype) && aligned4(dx, dtype) && aligned4(dout, dtype) &&
-                    aligned4(dgate, dtype) && aligned4(post_w, LEGO_F32) && aligned4(scale, LEGO_F32) && aligned4(next_w, LEGO_F32) && aligned4(workspace, LEGO_F32);
+    const bool full = width % 4 == 0;
     const int wgs = block_norm_grid(rows, wpr, bwd_cap(wpr));
     const dim3 grid(wgs), block(wpr == 16 ? 1024 : 256);
-#define GO(T, M, W, J, AL) hipLaunchKernelGGL((block_norm_bwd_kernel<T, M, W, J, AL>), grid, block, 0, ST, p, gy, gn, stat, (T*)dx, (T*)dout, (T*)dgate, workspace)
+#define GO(T, M, W, J, F) hipLaunchKernelGGL((block_norm_bwd_kernel<T, M, W, J, F>), grid, block, 0, ST, p, gy, gn, stat, (T*)dx, (T*)dout, (T*)dgate, workspace)
     LEGO_BY_TYPE(dtype, BY_MODE(GO, T));
 #undef GO
     if (int rc = check_launch("lego_block_norm_bwd")) return rc;
-    hipLaunchKernelGGL(block_norm_weights_kernel, dim3((width + 15) / 16), dim3(256), 0, ST, workspace, wgs, mode, post_w, scale, dpost_w, dscale, dnext_w, width);
+    hipLaunchKernelGGL(block_norm_weights_kernel, dim3((width + 15) / 16), dim3(1024), 0, ST, workspace, wgs, mode, post_w, scale, dpost_w, dscale, dnext_w, width);
     return check_launch("lego_block_norm_bwd (weights)");
 }

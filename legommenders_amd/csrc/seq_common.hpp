@@ -1,45 +1,63 @@
-// Shared by the sequence operators (scan_ops.hip, blocknorm_ops.hip, logprob_ops.hip): activations in fp32 / bf16 / fp16, four consecutive
-// channels a lane, every sum, statistic and state in fp32; one rounding to the activations' type, at the store.
+// Shared by the sequence operators (scan_ops.hip, blocknorm_ops.hip, logprob_ops.hip): activations in fp32 / bf16 / fp16, a few
+// consecutive channels a lane, every sum, statistic and state in fp32; one rounding to the activations' type, at the store.
 #pragma once
 #include "../../include/lego_hip.h"
 #include "common.hpp"
 
 namespace lego {
 
-template <typename T> using vec4 = T __attribute__((ext_vector_type(4)));
+template <typename T, int N> using vec = T __attribute__((ext_vector_type(N)));
 
-// channels c .. c + 3 of a row of `width`: one 16- / 8-byte load where the caller has shown the alignment (then width % 4 == 0), else one
-// load a channel; channels outside the row read as 0
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ f32x4 load4(const T* __restrict__ row, int c, int width) {
-    if constexpr (ALIGNED) {
-        if (c >= width) return f32x4{0.f, 0.f, 0.f, 0.f};
-        return __builtin_convertvector(*reinterpret_cast<const vec4<T>*>(row + c), f32x4);
-    } else {
-        f32x4 v;
+// Channels c .. c + N - 1 of a row of `width`, `at` bytes behind `base`; channels outside the row read as 0 and are not written.  `base` is the
+// same for the wave (scalar registers) and `at` a 32-bit lane offset: a 64-bit address a lane would cost two registers for every access.
+// Rows start anywhere (strides and odd widths leave 16-bit elements on 2-byte boundaries): the copies compile to ONE access at the element's
+// alignment, which the hardware takes; only a row's last lane, where `width` is no multiple of N (FULL = false), goes element by element.
+template <typename T, int N, bool FULL>
+__device__ __forceinline__ vec<T, N> load_raw(const T* __restrict__ base, uint32_t at, int c, int width) {
+    const T* p = reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + at);
+    vec<T, N> v;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = c + k < width ? (float)row[c + k] : 0.f;
-        return v;
+    for (int k = 0; k < N; ++k) v[k] = (T)0;
+    if (FULL ? c < width : c + N <= width) __builtin_memcpy(&v, p, sizeof(v));
+    else if (!FULL) {
+#pragma unroll
+        for (int k = 0; k < N - 1; ++k)
+            if (c + k < width) v[k] = p[k];
+    }
+    return v;
+}
+
+template <typename T, int N, bool FULL>
+__device__ __forceinline__ vec<float, N> load_at(const T* __restrict__ base, uint32_t at, int c, int width) {
+    return __builtin_convertvector((load_raw<T, N, FULL>(base, at, c, width)), vec<float, N>);
+}
+
+template <typename T, int N, bool FULL>
+__device__ __forceinline__ void store_at(T* __restrict__ base, uint32_t at, int c, int width, vec<float, N> v) {
+    T* p = reinterpret_cast<T*>(reinterpret_cast<char*>(base) + at);
+    const vec<T, N> o = __builtin_convertvector(v, vec<T, N>);
+    if (FULL ? c < width : c + N <= width) __builtin_memcpy(p, &o, sizeof(o));
+    else if (!FULL) {
+#pragma unroll
+        for (int k = 0; k < N - 1; ++k)
+            if (c + k < width) p[k] = o[k];
     }
 }
 
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void store4(T* __restrict__ row, int c, int width, f32x4 v) {
-    if constexpr (ALIGNED) {
-        if (c < width) *reinterpret_cast<vec4<T>*>(row + c) = __builtin_convertvector(v, vec4<T>);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (c + k < width) row[c + k] = (T)v[k];
-    }
+// the same of a row that begins at `row`
+template <typename T, int N, bool FULL>
+__device__ __forceinline__ vec<float, N> load(const T* __restrict__ row, int c, int width) {
+    return load_at<T, N, FULL>(row, (uint32_t)(c * (int)sizeof(T)), c, width);
+}
+template <typename T, int N, bool FULL>
+__device__ __forceinline__ void store(T* __restrict__ row, int c, int width, vec<float, N> v) {
+    store_at<T, N, FULL>(row, (uint32_t)(c * (int)sizeof(T)), c, width, v);
 }
 
 // 1 / (1 + e^-x) on the hardware exponential and reciprocal (each within 1 ulp); e^-x overflows to inf for x < -88 and gives 0
 __device__ __forceinline__ float sigmoid(float x) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * x));
 }
-
-inline bool aligned4(const void* p, int dtype) { return ((uintptr_t)p & (dtype == LEGO_F32 ? 15u : 7u)) == 0; }
 
 }  // namespace lego
 
