@@ -455,19 +455,20 @@ int lego_block_norm_bwd(const void* x, int64_t ldx, const void* o /*nullable*/, 
                         const void* dn, int64_t lddn, const float* stat, void* dx, void* dout, void* dgate, float* dpost_w, float* dscale,
                         float* dnext_w, float* workspace, int64_t workspace_floats, int rows, int width, void* stream);
 
-/* Log probabilities of rows of logits [rows, items]: lse, entropy, logp of `targets` (int32, or int64 with targets_64 = 1; outside [0, items)
- * or NULL: no target, logp 0), and the k <= LEGO_LOGPROBS_MAX_K largest log probabilities with their indices, largest first, equal values by
- * index.  A row with no item left (all masked or -inf) has lse, logp and top -inf, entropy 0 and indices -1; ranks behind the last item are
- * (-inf, -1); a row with NaN or +inf has NaN everywhere and indices -1.  mask_ld 0: one mask for all rows.
+/* Log probabilities of rows of logits [rows, items]: logp of `targets` (int32, or int64 with targets_64 = 1; outside [0, items) or NULL: no
+ * target, logp 0), the entropy, and the k <= LEGO_LOGPROBS_MAX_K largest log probabilities with their indices, largest first, equal values by
+ * index.  stat [rows, 2]: the maximum and ln of the sum of exp(x - maximum), whose sum is the log-sum-exp.  A row with no item left (all masked
+ * or -inf) has logp and top -inf, entropy 0, indices -1 and stat (-inf, 0); ranks behind the last item are (-inf, -1); a row with NaN or +inf has
+ * NaN for every number and indices -1.  mask_ld 0: one mask for all rows.
  * _bwd: dlogits [rows, items] (contiguous; 0 at masked places and in rows with nothing left) of g_logp, g_entropy [rows] and g_top [rows, k]
- * (each NULL = zeros), from lse, entropy and index of _fwd. */
+ * (each NULL = zeros), from stat, entropy and index of _fwd. */
 #define LEGO_LOGPROBS_MAX_K 128
-int64_t lego_token_logprobs_workspace(int rows, int items, int dtype, int k);    /* 8-byte words, for _fwd */
+int64_t lego_token_logprobs_workspace(int rows, int items, int dtype, int k);    /* 8-byte words (16-byte aligned), for _fwd */
 int lego_token_logprobs_fwd(const void* logits, int64_t ld, int dtype, const uint8_t* mask /*nullable*/, int64_t mask_ld, const void* targets,
-                            int targets_64, int k, float* logp, float* entropy, float* lse, float* top, int32_t* index, uint64_t* workspace,
+                            int targets_64, int k, float* logp, float* entropy, float* stat, float* top, int32_t* index, uint64_t* workspace,
                             int64_t workspace_words, int rows, int items, void* stream);
 int lego_token_logprobs_bwd(const void* logits, int64_t ld, int dtype, const uint8_t* mask /*nullable*/, int64_t mask_ld, const void* targets,
-                            int targets_64, int k, const float* lse, const float* entropy, const int32_t* index, const float* g_logp,
+                            int targets_64, int k, const float* stat, const float* entropy, const int32_t* index, const float* g_logp,
                             const float* g_entropy, const float* g_top, void* dlogits, int rows, int items, void* stream);
 
 /* small utilities used by the host side */

@@ -4,8 +4,9 @@
 //   oh = o (mean o^2 + eps)^-1/2      y = x + scale act(gate) oh post_w      yh = y (mean y^2 + eps)^-1/2      n = yh next_w
 //
 // in one pass: x, o and gate are read once, y and n written once.  Without a block (o = NULL) y = x and only n is written.  HBM-bound: a row
-// lives in the registers of 1, 4 or 16 waves (16- / 8-byte loads, 4 channels a lane), the weights of a lane's channels stay in registers over
-// the rows of a persistent workgroup.
+// lives in the registers of 1 to 16 waves (16- / 8-byte loads, 4 channels a lane), the weights of a lane's channels stay in registers over the rows
+// of a persistent workgroup, and the next row's loads are in flight while a row is summed -- without that the two dependent sums of a row left the
+// memory idle (65536 x 1024 bf16, backward: 454 us, 222 with it; 4.8 TB/s, as a copy of that size).
 //
 // Backward, with d = dy + rms_y^-1 (dn next_w - yh mean(dn next_w yh)) the gradient of y:  dx = d,  e = d scale act post_w,
 //   do = rms_o^-1 (e - oh mean(e oh)),  dgate = d scale oh post_w act'(gate),
@@ -42,7 +43,7 @@ __device__ __forceinline__ float gate_act(int act, float g, float& slope) {
 // sum over the row's waves; `red` is one of two buffers in turn, so that one barrier a sum is enough
 template <int WPR>
 __device__ __forceinline__ float row_sum(float v, float (*red)[16], int& turn) {
-    v = wave_sum(v);
+    v = wave_total(v);
     if constexpr (WPR > 1) {
         if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = v;
         __syncthreads();
@@ -54,13 +55,42 @@ __device__ __forceinline__ float row_sum(float v, float (*red)[16], int& turn) {
     return v;
 }
 
+// a lane's channels of a row's tensors, as they lie in memory
+template <typename T, int N, int NJ, bool FULL>
+struct Line {
+    vec<T, 4> v[N][NJ];
+    __device__ __forceinline__ void fetch(const Rows (&src)[N], int64_t row, int c0, int width) {
+#pragma unroll
+        for (int q = 0; q < N; ++q)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) v[q][j] = load_some<T, 4, FULL>((const T*)src[q].p + row * src[q].ld, c0 + 256 * j, width);
+    }
+    __device__ __forceinline__ f32x4 at(int q, int j) const { return __builtin_convertvector(v[q][j], f32x4); }
+};
+
+// the sum of a lane's 4 channels of f, without those behind the row
+template <bool FULL>
+__device__ __forceinline__ float in_row(f32x4 f, int c, int width) {
+    if constexpr (FULL) return c < width ? (f[0] + f[1]) + (f[2] + f[3]) : 0.f;
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s += c + k < width ? f[k] : 0.f;
+    return s;
+}
+
+template <int WPR> constexpr int kWaves = WPR == 1 ? 4 : WPR;          // one-wave rows: four of them a workgroup
+
 template <typename T, int MODE, int WPR, int NJ, bool FULL>
-__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_fwd_kernel(BlockNorm p, T* __restrict__ y, T* __restrict__ next, float* __restrict__ stat) {
+__global__ __launch_bounds__(64 * kWaves<WPR>) void block_norm_fwd_kernel(BlockNorm p, T* __restrict__ y, T* __restrict__ next, float* __restrict__ stat) {
     __shared__ float red[2][16];
     constexpr int RPW = WPR == 1 ? 4 : 1;                              // rows a workgroup holds at a time
+    constexpr int N = MODE & BN_BLOCK ? 3 : 1;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int c0 = 4 * (lane + (WPR == 1 ? 0 : 64 * NJ * wave)), W = p.width;
     const float inv = 1.f / (float)W;
+    Rows src[N];
+    src[0] = p.x;
+    if constexpr (MODE & BN_BLOCK) { src[1] = p.o; src[2] = p.act != 0 ? p.gate : p.x; }
     f32x4 wp[NJ], ws[NJ], wn[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
@@ -69,32 +99,28 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_fwd_kernel(
         if constexpr (MODE & BN_NEXT) wn[j] = load<float, 4, FULL>(p.next_w, c, W);
     }
     int turn = 0;
-    for (int64_t row = (int64_t)blockIdx.x * RPW + (WPR == 1 ? wave : 0); row < p.rows; row += (int64_t)gridDim.x * RPW) {
-        f32x4 v[NJ], ov[NJ], gv[NJ];
+    const int64_t step = (int64_t)gridDim.x * RPW;
+    int64_t row = (int64_t)blockIdx.x * RPW + (WPR == 1 ? wave : 0);
+    Line<T, N, NJ, FULL> in, ahead;
+    in.fetch(src, row < p.rows ? row : p.rows - 1, c0, W);
+    for (; row < p.rows; row += step) {
+        ahead.fetch(src, row + step < p.rows ? row + step : p.rows - 1, c0, W);
+        f32x4 v[NJ];
         float s = 0.f;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const int c = c0 + 256 * j;
-            if constexpr (MODE & BN_BLOCK) {
-                ov[j] = load<T, 4, FULL>((const T*)p.o.p + row * p.o.ld, c, W);
-                if (p.act != 0) gv[j] = load<T, 4, FULL>((const T*)p.gate.p + row * p.gate.ld, c, W);
-            }
-            v[j] = load<T, 4, FULL>((const T*)p.x.p + row * p.x.ld, c, W);
-        }
+        for (int j = 0; j < NJ; ++j) v[j] = in.at(0, j);
         if constexpr (MODE & BN_BLOCK) {
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s += ov[j][k] * ov[j][k];
+            for (int j = 0; j < NJ; ++j) s += in_row<FULL>(in.at(1, j) * in.at(1, j), c0 + 256 * j, W);
             const float ro = rsqrtf(row_sum<WPR>(s, red, turn) * inv + p.eps);
-            if (stat != nullptr && lane == 0 && (WPR == 1 || wave == 0)) stat[row] = ro;
+            if (stat != nullptr && threadIdx.x % (64 * WPR) == 0) stat[row] = ro;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
+                const f32x4 o = in.at(1, j), g = in.at(2, j);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     float slope;
-                    const float act = gate_act(p.act, p.act != 0 ? gv[j][k] : 0.f, slope);
-                    v[j][k] += ws[j][k] * act * (ov[j][k] * ro * wp[j][k]);
+                    v[j][k] += ws[j][k] * gate_act(p.act, g[k], slope) * (o[k] * ro * wp[j][k]);
                 }
                 store<T, 4, FULL>(y + row * W, c0 + 256 * j, W, v[j]);
             }
@@ -102,27 +128,34 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_fwd_kernel(
         if constexpr (MODE & BN_NEXT) {
             s = 0.f;
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s += v[j][k] * v[j][k];
+            for (int j = 0; j < NJ; ++j) s += in_row<FULL>(v[j] * v[j], c0 + 256 * j, W);
             const float ry = rsqrtf(row_sum<WPR>(s, red, turn) * inv + p.eps);
-            if (stat != nullptr && lane == 0 && (WPR == 1 || wave == 0)) stat[(MODE & BN_BLOCK ? p.rows : 0) + row] = ry;
+            if (stat != nullptr && threadIdx.x % (64 * WPR) == 0) stat[(MODE & BN_BLOCK ? p.rows : 0) + row] = ry;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) store<T, 4, FULL>(next + row * W, c0 + 256 * j, W, v[j] * ry * wn[j]);
         }
+        in = ahead;
     }
 }
 
 template <typename T, int MODE, int WPR, int NJ, bool FULL>
-__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_bwd_kernel(BlockNorm p, Rows dy, Rows dn, const float* __restrict__ stat,
-                                                                               T* __restrict__ dx, T* __restrict__ dout, T* __restrict__ dgate,
-                                                                               float* __restrict__ parts) {
+__global__ __launch_bounds__(64 * kWaves<WPR>) void block_norm_bwd_kernel(BlockNorm p, Rows dy, Rows dn, const float* __restrict__ stat,
+                                                                         T* __restrict__ dx, T* __restrict__ dout, T* __restrict__ dgate,
+                                                                         float* __restrict__ parts) {
     __shared__ float red[2][16];
     constexpr int RPW = WPR == 1 ? 4 : 1;
+    constexpr int N = MODE == (BN_BLOCK | BN_NEXT) ? 5 : 3;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int c0 = 4 * (lane + (WPR == 1 ? 0 : 64 * NJ * wave)), W = p.width;
     const float inv = 1.f / (float)W;
     const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+    // what a row reads: dy first (any tensor in its place where there is none), then x and dn of the norm, o and the gate of the block
+    constexpr int X = 1, DN = 2, O = MODE & BN_NEXT ? 3 : 1, G = O + 1;
+    const bool has_dy = dy.p != nullptr;
+    Rows src[N];
+    src[0] = has_dy ? dy : p.x;
+    if constexpr (MODE & BN_NEXT) { src[X] = p.x; src[DN] = dn; }
+    if constexpr (MODE & BN_BLOCK) { src[O] = p.o; src[G] = p.act != 0 ? p.gate : p.o; }
     f32x4 wp[NJ], ws[NJ], wn[NJ], z[NJ], zn[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
@@ -132,42 +165,42 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_bwd_kernel(
         z[j] = zn[j] = zero;
     }
     int turn = 0;
-    for (int64_t row = (int64_t)blockIdx.x * RPW + (WPR == 1 ? wave : 0); row < p.rows; row += (int64_t)gridDim.x * RPW) {
-        f32x4 v[NJ], oh[NJ], gv[NJ], d[NJ], t[NJ];
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const int c = c0 + 256 * j;
-            d[j] = dy.p != nullptr ? load<T, 4, FULL>((const T*)dy.p + row * dy.ld, c, W) : zero;
-            if constexpr (MODE & BN_BLOCK) {
-                oh[j] = load<T, 4, FULL>((const T*)p.o.p + row * p.o.ld, c, W);
-                gv[j] = p.act != 0 ? load<T, 4, FULL>((const T*)p.gate.p + row * p.gate.ld, c, W) : zero;
-            }
-            if constexpr (MODE & BN_NEXT) {
-                v[j] = load<T, 4, FULL>((const T*)p.x.p + row * p.x.ld, c, W);
-                t[j] = load<T, 4, FULL>((const T*)dn.p + row * dn.ld, c, W);
-            }
-        }
+    const int64_t step = (int64_t)gridDim.x * RPW;
+    int64_t row = (int64_t)blockIdx.x * RPW + (WPR == 1 ? wave : 0);
+    Line<T, N, NJ, FULL> in, ahead;
+    in.fetch(src, row < p.rows ? row : p.rows - 1, c0, W);
+    for (; row < p.rows; row += step) {
+        const float ro = MODE & BN_BLOCK ? stat[row] : 0.f, ry = MODE & BN_NEXT ? stat[(MODE & BN_BLOCK ? p.rows : 0) + row] : 0.f;
+        ahead.fetch(src, row + step < p.rows ? row + step : p.rows - 1, c0, W);
+        f32x4 oh[NJ], act[NJ], slope[NJ], d[NJ], t[NJ];
         if constexpr (MODE & BN_BLOCK) {
-            const float ro = stat[row];
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) oh[j] *= ro;
-        }
-        if constexpr (MODE & BN_NEXT) {
-            const float ry = stat[(MODE & BN_BLOCK ? p.rows : 0) + row];
-            float s = 0.f;
-#pragma unroll
-            for (int j = 0; j < NJ; ++j)
+            for (int j = 0; j < NJ; ++j) {
+                const f32x4 g = in.at(G, j);
+                oh[j] = in.at(O, j) * ro;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    if constexpr (MODE & BN_BLOCK) {
-                        float slope;
-                        v[j][k] += ws[j][k] * gate_act(p.act, gv[j][k], slope) * (oh[j][k] * wp[j][k]);
-                    }
-                    v[j][k] *= ry;                                     // yh
-                    zn[j][k] += t[j][k] * v[j][k];
-                    t[j][k] *= wn[j][k];
-                    s += t[j][k] * v[j][k];
+                    float sl;
+                    act[j][k] = gate_act(p.act, g[k], sl);
+                    slope[j][k] = sl;
                 }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) d[j] = has_dy ? in.at(0, j) : zero;
+        if constexpr (MODE & BN_NEXT) {
+            f32x4 v[NJ];
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const f32x4 g = in.at(DN, j);
+                v[j] = in.at(X, j);
+                if constexpr (MODE & BN_BLOCK) v[j] += ws[j] * act[j] * (oh[j] * wp[j]);
+                v[j] *= ry;                                            // yh
+                zn[j] += g * v[j];
+                t[j] = g * wn[j];
+                s += in_row<FULL>(t[j] * v[j], c0 + 256 * j, W);
+            }
             const float m = row_sum<WPR>(s, red, turn) * inv;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) d[j] += ry * (t[j] - v[j] * m);
@@ -178,23 +211,17 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void block_norm_bwd_kernel(
             float s = 0.f;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-                f32x4 dg;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float slope;
-                    const float act = gate_act(p.act, gv[j][k], slope);
-                    z[j][k] += d[j][k] * act * oh[j][k];
-                    const float e = d[j][k] * ws[j][k];
-                    dg[k] = e * oh[j][k] * wp[j][k] * slope;
-                    t[j][k] = e * act * wp[j][k];
-                    s += t[j][k] * oh[j][k];
-                }
-                if (p.act != 0) store<T, 4, FULL>(dgate + row * W, c0 + 256 * j, W, dg);
+                z[j] += d[j] * act[j] * oh[j];
+                const f32x4 e = d[j] * ws[j] * wp[j];
+                t[j] = e * act[j];
+                s += in_row<FULL>(t[j] * oh[j], c0 + 256 * j, W);
+                if (p.act != 0) store<T, 4, FULL>(dgate + row * W, c0 + 256 * j, W, e * oh[j] * slope[j]);
             }
-            const float m = row_sum<WPR>(s, red, turn) * inv, ro = stat[row];
+            const float m = row_sum<WPR>(s, red, turn) * inv;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) store<T, 4, FULL>(dout + row * W, c0 + 256 * j, W, ro * (t[j] - oh[j] * m));
         }
+        in = ahead;
     }
     // this workgroup's partial column sums: parts[workgroup][0] = z, [1] = zn
     float* mine = parts + (int64_t)blockIdx.x * 2 * W;
@@ -251,10 +278,12 @@ __global__ __launch_bounds__(1024) void block_norm_weights_kernel(const float* _
     }
 }
 
-// waves a row and 4-channel groups a lane: one wave to 1024 channels, then 4 (to 4096), then 16 (to 16384)
+// Waves a row and 4-channel groups a lane: one wave to 1024 channels (no barrier in its sums), then 4, 8 and 16 waves of two groups, as many lanes as
+// the width needs; four groups in 16 waves above 8192.  Measured backwards, bf16, TB/s: 1024 channels in 1 x 4 / 2 x 2 / 4 x 1 (waves x groups)
+// 4.8 / 3.9-5.1 / 4.7-5.1, 512 channels in 1 x 2 / 2 x 1 5.1 / 2.9-4.7, 4096 channels in 8 x 2 / 16 x 1 4.8 / 4.8.
 static void block_norm_shape(int width, int& wpr, int& nj) {
-    wpr = width <= 1024 ? 1 : width <= 4096 ? 4 : 16;
-    nj = (width + 256 * wpr - 1) / (256 * wpr);
+    wpr = width <= 1024 ? 1 : width <= 2048 ? 4 : width <= 4096 ? 8 : 16;
+    nj = wpr == 1 ? (width + 255) / 256 : width <= 8192 ? 2 : 4;
 }
 
 static int block_norm_grid(int rows, int wpr, int cap) {
@@ -263,8 +292,9 @@ static int block_norm_grid(int rows, int wpr, int cap) {
     return (int)(wgs < cap ? wgs : cap);
 }
 
-constexpr int BN_FWD_CAP = 2048;
-static int bwd_cap(int wpr) { return wpr == 16 ? 256 : 1024; }
+// workgroups at most (they then take rows in turn): forward 2048 -- 4096 and 1024 are 2 to 6 % slower at 29600 x 768 fp32 --, backward 512, where
+// more cost partial rows of column sums and weights that are loaded again (65536 x 512 bf16: 104 us, 125 with 1024)
+constexpr int BN_FWD_CAP = 2048, BN_BWD_CAP = 512;
 
 }  // namespace lego
 
@@ -274,11 +304,14 @@ using namespace lego;
 // one instantiation for the row's shape; widths that are no multiple of 4 take the widest form of their wave count
 #define BY_SHAPE(GO, T, MODE)                                                                                                                      \
     do {                                                                                                                                           \
-        if (!full) { if (wpr == 1) GO(T, MODE, 1, 4, false); else if (wpr == 4) GO(T, MODE, 4, 4, false); else GO(T, MODE, 16, 4, false); }           \
+        if (!full) { if (wpr == 1) GO(T, MODE, 1, 4, false); else if (wpr == 4) GO(T, MODE, 4, 2, false);                                           \
+                     else if (wpr == 8) GO(T, MODE, 8, 2, false); else GO(T, MODE, 16, 4, false); }                                                 \
         else if (wpr == 1) { if (nj == 1) GO(T, MODE, 1, 1, true); else if (nj == 2) GO(T, MODE, 1, 2, true);                                       \
                              else if (nj == 3) GO(T, MODE, 1, 3, true); else GO(T, MODE, 1, 4, true); }                                             \
-        else if (wpr == 4) { if (nj == 2) GO(T, MODE, 4, 2, true); else GO(T, MODE, 4, 4, true); }                                                  \
-        else { if (nj == 2) GO(T, MODE, 16, 2, true); else GO(T, MODE, 16, 4, true); }                                                              \
+        else if (wpr == 4) GO(T, MODE, 4, 2, true);                                                                                                \
+        else if (wpr == 8) GO(T, MODE, 8, 2, true);                                                                                                \
+        else if (nj == 2) GO(T, MODE, 16, 2, true);                                                                                                \
+        else GO(T, MODE, 16, 4, true);                                                                                                             \
     } while (0)
 #define BY_MODE(GO, T) do { if (mode == 3) BY_SHAPE(GO, T, 3); else if (mode == BN_BLOCK) BY_SHAPE(GO, T, 1); else BY_SHAPE(GO, T, 2); } while (0)
 
@@ -297,7 +330,7 @@ extern "C" int64_t lego_block_norm_workspace(int rows, int width) {
     if (rows <= 0 || width <= 0) return 0;
     int wpr, nj;
     block_norm_shape(width, wpr, nj);
-    return (int64_t)block_norm_grid(rows, wpr, bwd_cap(wpr)) * 2 * width;
+    return (int64_t)block_norm_grid(rows, wpr, BN_BWD_CAP) * 2 * width;
 }
 
 extern "C" int lego_block_norm_fwd(const void* x, int64_t ldx, const void* o, int64_t ldo, const void* gate, int64_t ldg, int dtype, int act,
@@ -311,7 +344,7 @@ extern "C" int lego_block_norm_fwd(const void* x, int64_t ldx, const void* o, in
     int wpr, nj;
     block_norm_shape(width, wpr, nj);
     const bool full = width % 4 == 0;
-    const dim3 grid(block_norm_grid(rows, wpr, BN_FWD_CAP)), block(wpr == 16 ? 1024 : 256);
+    const dim3 grid(block_norm_grid(rows, wpr, BN_FWD_CAP)), block(64 * (wpr == 1 ? 4 : wpr));
 #define GO(T, M, W, J, F) hipLaunchKernelGGL((block_norm_fwd_kernel<T, M, W, J, F>), grid, block, 0, ST, p, (T*)y, (T*)next, stat)
     LEGO_BY_TYPE(dtype, BY_MODE(GO, T));
 #undef GO
@@ -335,8 +368,8 @@ extern "C" int lego_block_norm_bwd(const void* x, int64_t ldx, const void* o, in
     block_norm_shape(width, wpr, nj);
     const Rows gy{dy, lddy}, gn{dn, lddn};
     const bool full = width % 4 == 0;
-    const int wgs = block_norm_grid(rows, wpr, bwd_cap(wpr));
-    const dim3 grid(wgs), block(wpr == 16 ? 1024 : 256);
+    const int wgs = block_norm_grid(rows, wpr, BN_BWD_CAP);
+    const dim3 grid(wgs), block(64 * (wpr == 1 ? 4 : wpr));
 #define GO(T, M, W, J, F) hipLaunchKernelGGL((block_norm_bwd_kernel<T, M, W, J, F>), grid, block, 0, ST, p, gy, gn, stat, (T*)dx, (T*)dout, (T*)dgate, workspace)
     LEGO_BY_TYPE(dtype, BY_MODE(GO, T));
 #undef GO

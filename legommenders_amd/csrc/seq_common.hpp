@@ -59,6 +59,33 @@ __device__ __forceinline__ float sigmoid(float x) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * x));
 }
 
+// the sum over the wave's 64 lanes, in every lane: shifts inside rows of 16 lanes, then across the rows, on the vector unit alone
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float add_shifted(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xF, true));
+}
+__device__ __forceinline__ float wave_total(float v) {
+    v = add_shifted<0x111, 0xF>(v);                                    // row_shr:1, 2, 4, 8
+    v = add_shifted<0x112, 0xF>(v);
+    v = add_shifted<0x114, 0xF>(v);
+    v = add_shifted<0x118, 0xF>(v);
+    v = add_shifted<0x142, 0xA>(v);                                    // row_bcast:15 into rows 1 and 3, row_bcast:31 into rows 2 and 3
+    v = add_shifted<0x143, 0xC>(v);
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// Channels c .. c + N - 1 of a row without a branch, for kernels that keep the next rows' loads in flight: channels behind the row read its end
+// again (the caller leaves them out of its sums and does not store them).
+template <typename T, int N, bool FULL>
+__device__ __forceinline__ vec<T, N> load_some(const T* __restrict__ row, int c, int width) {
+    vec<T, N> v;
+    if constexpr (FULL) __builtin_memcpy(&v, row + min(c, width - N), sizeof(v));
+    else
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = row[min(c + k, width - 1)];
+    return v;
+}
+
 }  // namespace lego
 
 // one instantiation of BODY for the activations' type, named T there

@@ -414,22 +414,22 @@ def block_norm_bwd(dy, dn, x, o, gate, post_w, scale, next_w, eps, act, stat):
 
 
 def token_logprobs_fwd(logits, targets, k=0, mask=None):
-    """2-D logits -> logp, entropy, lse [rows], top [rows, k] fp32, index [rows, k] int32"""
+    """2-D logits -> logp, entropy [rows], stat [rows, 2] (maximum, ln of the sum), top [rows, k] fp32, index [rows, k] int32"""
     rows, items = logits.shape
     f = dict(dtype=torch.float32, device=logits.device)
-    logp, entropy, lse = torch.empty(rows, **f), torch.empty(rows, **f), torch.empty(rows, **f)
+    logp, entropy, stat = torch.empty(rows, **f), torch.empty(rows, **f), torch.empty(rows, 2, **f)
     top, index = torch.empty(rows, k, **f), torch.empty(rows, k, dtype=torch.int32, device=logits.device)
     logits, mask = _last_dense(logits), _bytes(mask)
     targets = None if targets is None else targets.contiguous()
     size = _lib.lib().lego_token_logprobs_workspace(rows, items, _DTYPES[logits.dtype], k)
     ws = _floats(size, logits.device, torch.int64)
     _launch(logits, "lego_token_logprobs_fwd", _at(logits), logits.stride(0), _DTYPES[logits.dtype], _at(mask), 0 if mask is None else mask.stride(0),
-         _at(targets), int(targets is not None and targets.dtype == torch.int64), k, _at(logp), _at(entropy), _at(lse), _at(top),
+         _at(targets), int(targets is not None and targets.dtype == torch.int64), k, _at(logp), _at(entropy), _at(stat), _at(top),
          _at(index), _at(ws), size, rows, items)
-    return logp, entropy, lse, top, index
+    return logp, entropy, stat, top, index
 
 
-def token_logprobs_bwd(g_logp, g_entropy, g_top, logits, targets, mask, lse, entropy, index):
+def token_logprobs_bwd(g_logp, g_entropy, g_top, logits, targets, mask, stat, entropy, index):
     """-> d logits [rows, items], in their type; a gradient that is None counts as zeros"""
     rows, items = logits.shape
     out = torch.empty(rows, items, dtype=logits.dtype, device=logits.device)
@@ -438,6 +438,6 @@ def token_logprobs_bwd(g_logp, g_entropy, g_top, logits, targets, mask, lse, ent
     if g_top is not None and g_top.numel() == 0:
         g_top = None
     _launch(logits, "lego_token_logprobs_bwd", _at(logits), logits.stride(0), _DTYPES[logits.dtype], _at(mask), 0 if mask is None else mask.stride(0),
-         _at(targets), int(targets is not None and targets.dtype == torch.int64), index.shape[1], _at(lse), _at(entropy), _at(index),
+         _at(targets), int(targets is not None and targets.dtype == torch.int64), index.shape[1], _at(stat), _at(entropy), _at(index),
          _at(g_logp), _at(g_entropy), _at(g_top), _at(out), rows, items)
     return out

@@ -620,36 +620,36 @@ class BlockNorm(torch.autograd.Function):
 _differentiable("block_norm", BlockNorm, range(6))
 
 
-# ---- token_logprobs: rows of logits [rows, items] -> (log probability of the target, entropy, log-sum-exp, the k largest log probabilities, their
-# indices)
+# ---- token_logprobs: rows of logits [rows, items] -> (log probability of the target, entropy, [rows, 2] maximum and ln of the sum of
+# exp(x - maximum), the k largest log probabilities, their indices)
 def _lp_fake(logits, targets, mask, k):
     rows, f = logits.shape[0], dict(dtype=torch.float32)
-    return (logits.new_empty(rows, **f), logits.new_empty(rows, **f), logits.new_empty(rows, **f), logits.new_empty(rows, k, **f),
+    return (logits.new_empty(rows, **f), logits.new_empty(rows, **f), logits.new_empty(rows, 2, **f), logits.new_empty(rows, k, **f),
             logits.new_empty(rows, k, dtype=torch.int32))
 
 
 logprobs_op = _define("token_logprobs", "(Tensor logits, Tensor? targets, Tensor? mask, SymInt k) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
               lambda logits, targets, mask, k: K.token_logprobs_fwd(logits, targets, k, mask), _lp_fake)
-logprobs_bwd_op = _define("token_logprobs_bwd", "(Tensor? g_logp, Tensor? g_entropy, Tensor? g_top, Tensor logits, Tensor? targets, Tensor? mask, Tensor lse,"
+logprobs_bwd_op = _define("token_logprobs_bwd", "(Tensor? g_logp, Tensor? g_entropy, Tensor? g_top, Tensor logits, Tensor? targets, Tensor? mask, Tensor stat,"
                   " Tensor entropy, Tensor index) -> Tensor", K.token_logprobs_bwd,
-                  lambda g_logp, g_entropy, g_top, logits, targets, mask, lse, entropy, index: logits.new_empty(logits.shape))
+                  lambda g_logp, g_entropy, g_top, logits, targets, mask, stat, entropy, index: logits.new_empty(logits.shape))
 
 
 class TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, mask, k):
         with below_autograd():
-            logp, entropy, lse, top, index = logprobs_op(logits, targets, mask, k)
-        ctx.save_for_backward(logits, targets, mask, lse, entropy, index)
-        ctx.mark_non_differentiable(lse, index)
+            logp, entropy, stat, top, index = logprobs_op(logits, targets, mask, k)
+        ctx.save_for_backward(logits, targets, mask, stat, entropy, index)
+        ctx.mark_non_differentiable(stat, index)
         ctx.set_materialize_grads(False)
-        return logp, entropy, lse, top, index
+        return logp, entropy, stat, top, index
 
     @staticmethod
-    def backward(ctx, g_logp, g_entropy, g_lse, g_top, g_index):
+    def backward(ctx, g_logp, g_entropy, g_stat, g_top, g_index):
         _once("lego_hip::token_logprobs")
-        logits, targets, mask, lse, entropy, index = ctx.saved_tensors
-        return logprobs_bwd_op(g_logp, g_entropy, g_top, logits, targets, mask, lse, entropy, index), None, None, None
+        logits, targets, mask, stat, entropy, index = ctx.saved_tensors
+        return logprobs_bwd_op(g_logp, g_entropy, g_top, logits, targets, mask, stat, entropy, index), None, None, None
 
 
 _differentiable("token_logprobs", TokenLogprobs, (0,))

@@ -205,7 +205,7 @@ def test_shapes_without_a_gpu():
         y, n, stat = L.block_norm(x[0], x[0], x[0], lam, lam, None, 1e-6, 2, False)
         assert y.shape == (130, 24) and n.numel() == 0 and stat.shape == (1, 0)
         out = L.token_logprobs(x[0], None, None, 5)
-        assert [tuple(t.shape) for t in out] == [(130,), (130,), (130,), (130, 5), (130, 5)] and out[4].dtype == torch.int32
+        assert [tuple(t.shape) for t in out] == [(130,), (130,), (130, 2), (130, 5), (130, 5)] and out[4].dtype == torch.int32
 
 
 # --------------------------------------------------------------------------------------------------------------- GPU: the recurrence
@@ -639,7 +639,7 @@ def test_opcheck(name):
     mask = torch.ones(2, 70, dtype=torch.bool, device="cuda")
     a, b, c = (t.view(-1, 12) for t in (x, r, i))
     req = lambda *ts: tuple(t.clone().requires_grad_() for t in ts)      # noqa: E731
-    lse, ent = torch.zeros(140, device="cuda"), torch.zeros(140, device="cuda")
+    ent = torch.zeros(140, device="cuda")
     args = {
         "gated_scan": (*req(x, r, i, lam), mask, *req(st), 8.0, True),
         "gated_scan_bwd": (x, st, x, r, i, lam, mask, torch.zeros(2, 2, 12, device="cuda"), 8.0),
@@ -648,7 +648,7 @@ def test_opcheck(name):
         "block_norm_plain": (*req(a), None, None, None, None, *req(w), 1e-6, 0, True),
         "block_norm_bwd": (a, b, a, b, c, w, w, w, torch.ones(2, 140, device="cuda"), 1e-6, 2),
         "token_logprobs": (*req(a), torch.zeros(140, dtype=torch.int64, device="cuda"), None, 3),
-        "token_logprobs_bwd": (lse, ent, None, a, torch.zeros(140, dtype=torch.int64, device="cuda"), None, lse, ent,
+        "token_logprobs_bwd": (ent, ent, None, a, torch.zeros(140, dtype=torch.int64, device="cuda"), None, torch.zeros(140, 2, device="cuda"), ent,
                                torch.zeros(140, 3, dtype=torch.int32, device="cuda")),
     }[name]
     torch.library.opcheck(getattr(L, name.replace("_plain", "")).default, args,
@@ -751,7 +751,7 @@ def test_nothing_is_written_outside_the_outputs():
     logits = _rand(4, rows, items).cuda()
     size = _lib.lib().lego_token_logprobs_workspace(rows, items, 0, k)
     ws3, wp3 = banded(max(size, 1), torch.int64)
-    row = [banded(rows) for _ in range(3)] + [banded(rows * k), banded(rows * k, torch.int32)]
+    row = [banded(rows), banded(rows), banded(2 * rows)] + [banded(rows * k), banded(rows * k, torch.int32)]
     t = torch.zeros(rows, dtype=torch.int64, device="cuda")
     _lib.call("lego_token_logprobs_fwd", p(logits), items, 0, None, 0, p(t), 1, k, *(o[1] for o in row), wp3, size, rows, items, st)
     d = banded(rows * items)
