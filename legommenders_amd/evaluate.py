@@ -37,6 +37,39 @@ def gather_shards(local: torch.Tensor, n: int, process_group, world: int) -> tor
     return full[:n]
 
 
+@torch.no_grad()
+def next_items(user_repr, item_repr, users, targets=None, k=10, seen=None, page=512):
+    """What the users would click next, over the whole catalogue: scores <user, item> of every item, their softmax.
+
+    users [n] rows of user_repr; targets [n] items (optional; -1: none); seen (user_hist [n_users, S], user_hist_len [n_users]): clicks that are
+    left out of the catalogue (a target is always in).  -> dict of logp [n] of the targets, entropy [n], top [n, k] log probabilities and
+    items [n, k] int32 (-1 where nothing is left), `page` users at a time (their scores are [page, n_items] fp32)."""
+    from . import functional as F
+    dev, n_items = item_repr.device, item_repr.shape[0]
+    users = torch.as_tensor(users).to(dev, torch.int64)
+    if targets is not None:
+        targets = torch.as_tensor(targets).to(dev, torch.int64)
+    padded = torch.nn.functional.pad(item_repr, (0, 0, 0, -n_items % 4))                     # (the products' rows are multiples of 4 elements)
+    out = []
+    for s in range(0, users.numel(), page):
+        u = users[s:s + page]
+        t = None if targets is None else targets[s:s + page]
+        mask = None
+        if seen is not None:
+            hist, length = seen[0][u].long(), seen[1][u]
+            S = hist.shape[1]
+            mask = torch.ones(u.numel(), n_items + 1, dtype=torch.bool, device=dev)          # the last column takes the pads
+            mask.scatter_(1, torch.where(torch.arange(S, device=dev)[None] < length[:, None], hist, n_items), False)
+            if t is not None:
+                mask.scatter_(1, torch.where(t >= 0, t, n_items)[:, None], True)
+            mask = mask[:, :n_items]
+        out.append(F.token_logprobs(F.linear(user_repr[u], padded)[:, :n_items], t, k=k, mask=mask))
+    if not out:
+        empty = torch.empty(0, dtype=torch.float32, device=dev)
+        return dict(logp=empty, entropy=empty, top=empty.view(0, k), items=empty.view(0, k).to(torch.int32))
+    return {name: torch.cat([o[q] for o in out]) for q, name in enumerate(("logp", "entropy", "top", "items"))}
+
+
 class Evaluator:
     def __init__(self, kind, params, data, item_page=512, user_page=512, heads=8, glove=True, process_group=None,
                  rank=0, world_size=1):
@@ -85,6 +118,10 @@ class Evaluator:
         call("lego_gather_rows", _ptr(self.item_repr), D, D, _ptr(it), n, None, _ptr(gi), D, 0, st)
         call("lego_rowdot_fwd", _ptr(gu), D, _ptr(gi), D, n, D, _ptr(out), st)
         return out
+
+    def next_items(self, users, targets=None, k=10, exclude_seen=False):
+        """`next_items` on the cached vectors (build_caches first)"""
+        return next_items(self.user_repr, self.item_repr, users, targets, k, (self.data.user_hist, self.data.user_hist_len) if exclude_seen else None)
 
     def evaluate(self, users, items, labels, groups=None, metrics=("GAUC", "MRR", "NDCG@1", "NDCG@5", "NDCG@10")):
         """every rank calls this (the cache build holds the collectives); ranks other than 0 return ({}, None)"""

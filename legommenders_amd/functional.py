@@ -257,3 +257,21 @@ def token_logprobs(logits, targets=None, k=0, mask=None):
         return logp, entropy, top, index
     lead = logits.shape[:-1]
     return logp.view(lead), entropy.view(lead), top.view(*lead, k), index.view(*lead, k)
+
+
+def catalogue_scores(user, items):
+    """<user, item> of every pair: user [B, D] x items [N, D] -> [B, N] on the product kernels.  Their rows are multiples of 4 elements: other
+    catalogues are padded by zero items, and the result is a view without them (`token_logprobs` takes such rows)."""
+    n = items.shape[0]
+    return linear(user, torch.nn.functional.pad(items, (0, 0, 0, -n % 4)) if n % 4 else items)[:, :n]
+
+
+def next_item_loss(user, items, targets, mask=None):
+    """-mean log probability of each user's next item over a whole catalogue: user [B, D] x items [N, D] -> scalar; targets [B] (outside
+    [0, N): the row does not count).  The full-softmax sibling of `dot_ce`'s sampled one: the scores are one product, their softmax and its
+    gradient one pass each."""
+    if targets.dim() != 1 or user.dim() != 2 or targets.shape[0] != user.shape[0]:
+        _refuse("next_item_loss", f"targets are one item a user: {tuple(targets.shape)} for users {tuple(user.shape)}")
+    _need_gpu(user, "next_item_loss")
+    logp = token_logprobs(catalogue_scores(user, items), targets, mask=mask)[0]
+    return -logp.sum() / ((targets >= 0) & (targets < items.shape[0])).sum().clamp(min=1)

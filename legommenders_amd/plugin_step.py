@@ -259,6 +259,11 @@ class PluginEvaluator:
         call("lego_rowdot_fwd", _ptr(gu), D, _ptr(gi), D, n, D, _ptr(out), st)
         return out
 
+    def next_items(self, users, targets=None, k=10, exclude_seen=False):
+        """`evaluate.next_items` on the cached vectors (build_caches first)"""
+        from legommenders_amd.evaluate import next_items
+        return next_items(self.user_repr, self.item_repr, users, targets, k, (self.data.user_hist, self.data.user_hist_len) if exclude_seen else None)
+
     def evaluate(self, users, items, labels, groups=None, metrics=("GAUC", "MRR", "NDCG@1", "NDCG@5", "NDCG@10")):
         from legommenders_amd import metrics as M
         import numpy as np

@@ -4,6 +4,9 @@ evaluate the test split (`test`, result file next to the checkpoint) or time the
     python -m legommenders_amd.tester --data config/data/synthetic.yaml --model config/model/naml.yaml \
         --embed config/embed/glove.yaml --hidden_size 256 --batch_size 64 --load_sign <signature> [--latency --num_batches 1000]
 
+`--next_items K` scores the test split's clicked rows against the WHOLE catalogue instead of the rows' candidates: the mean log probability of the
+click, the mean entropy of the user's distribution and the share of clicks among its K likeliest items (no counterpart in the reference).
+
 What `--latency` times: the reference brackets `legommender(batch=batch)` of every test batch with
 `Env.latency_timer` (base_lego.py:373-381) -- with `use_fast_eval` that is the id-gather of the cached user / item
 vectors plus the dot (model/legommender.py:153-157,202-214,282); the caches are built before the loop and are not
@@ -75,7 +78,23 @@ class Tester(Trainer):
         self.log(f"Total {st.count} steps, avg ms {st.avgms():.4f}")
         return st
 
+    def next_items(self, k):
+        rows = self.world["test"]
+        self.evaluator.build_caches()                                       # every rank: the caches are built from all shards
+        if self.rank != 0:
+            return {}
+        hit = torch.as_tensor(rows["label"]) == 1
+        users, items = torch.as_tensor(rows["user"])[hit], torch.as_tensor(rows["item"])[hit]
+        r = self.evaluator.next_items(users, items, k=k)
+        found = (r["items"] == items.to(r["items"])[:, None]).any(1).float()
+        res = {"LogProb": float(r["logp"].mean()), "Entropy": float(r["entropy"].mean()), f"HitRatio@{k}": float(found.mean())}
+        for name, v in res.items():
+            self.log(f"{name}: {v:.4f}")
+        return res
+
     def run(self):
+        if self.config.next_items:
+            return self.next_items(int(self.config.next_items))
         if self.config.latency:
             return self.latency()
         return self.test()
@@ -85,7 +104,7 @@ def get_configurations(kwargs=None) -> Obj:
     return CommandInit(
         required_args=["data", "model"],
         default_args=dict(embed="config/embed/null.yaml", exp="config/exp/default.yaml", hidden_size=256,
-                          item_hidden_size="${hidden_size}$", latency=False, num_batches=1000),
+                          item_hidden_size="${hidden_size}$", latency=False, num_batches=1000, next_items=0),
     ).parse(kwargs=kwargs)
 
 
