@@ -3,22 +3,32 @@
 //   l_t = -c softplus(lam) sigmoid(r_t)      a_t = e^l_t      b_t = sqrt(1 - a_t^2) sigmoid(i_t) x_t       h_t = a_t h_(t-1) + b_t
 //
 // Steps compose: (A2, H2) after (A1, H1) is (A2 A1, A2 H1 + H2).  A workgroup owns 64 channels of one sequence and walks it in tiles of 64
-// steps: a lane holds 4 channels x 4 steps in registers, composes them, the 4 groups of a wave join by shuffles, the 4 waves through LDS
-// (one barrier a tile), and each lane then replays its 4 steps from the state that reaches it -- every input is read once.  Few sequences
+// steps: a lane holds 2 channels x a few steps in registers and composes them, the two halves of a wave join by a shuffle, the waves through LDS
+// (one barrier a tile), and each lane then replays its steps from the state that reaches it -- every input is read once.  Few sequences
 // that are long are cut into chunks: a first launch composes each chunk, the second starts every chunk from the chunks before it.
 //
 // The backward pass keeps no h: the forward pass saves the fp32 state at the head of every tile (1/64 of the cells), the tile's states are
 // formed again from it in fp32, and G_t = dh_t + a_(t+1) G_(t+1) is the same composition from the other end.
+//
+// What bounds it: memory from about 192 workgroups on (64 x 2048 x 256 fp32: forward 109 us, 4.9 TB/s; backward 217 us, 4.3 TB/s); in bf16, with half the
+// bytes, the exponentials and the waits of 16 waves a CU (forward 187 us for 2 x 32768 x 768, its inputs read twice: 3.8 TB/s).  512 x 50 x 256 fp32 with
+// ragged lengths: 19 us forward, 40 backward.
 #include <type_traits>
 
 #include "seq_common.hpp"
 
 namespace lego {
 
-// A lane holds SC_VC channels x SC_STEPS steps; SC_LANES lanes span the channels, the other lanes and the waves the tile's steps.
-constexpr int SC_VC = 2, SC_STEPS = 4, SC_LANES = 32, SC_WAVES = 8, SC_TILE = LEGO_SCAN_TILE;
-constexpr int SC_CH = SC_VC * SC_LANES, SC_GROUPS = 64 / SC_LANES, SC_RUNS = SC_GROUPS * SC_WAVES, SC_THREADS = 64 * SC_WAVES;
-static_assert(SC_TILE == SC_STEPS * SC_RUNS, "a tile is SC_RUNS runs of SC_STEPS steps");
+// A lane holds SC_VC channels x STEPS steps; SC_LANES lanes span the channels, the other lanes and the waves the tile's runs of STEPS steps.
+constexpr int SC_VC = 2, SC_LANES = 32, SC_TILE = LEGO_SCAN_TILE, SC_CH = SC_VC * SC_LANES, SC_GROUPS = 64 / SC_LANES;
+template <int WAVES_, int STEPS_> struct Shape {
+    static constexpr int WAVES = WAVES_, STEPS = STEPS_, RUNS = SC_GROUPS * WAVES, THREADS = 64 * WAVES;
+    static_assert(STEPS * RUNS == SC_TILE && SC_VC == 2, "a tile is RUNS runs of STEPS steps");
+};
+// Measured (us): forward 8 x 4 / 4 x 8, 64 x 2048 x 256 fp32 115 / 117, 1 x 10007 x 301 fp16 42 / 48; backward, which has the registers of 16 cells a
+// lane only in workgroups of 4 waves, 512 x 50 x 256 fp32 84 / 54, 64 x 2048 x 256 fp32 231 / 211.
+using Fwd = Shape<8, 4>;
+using Bwd = Shape<4, 8>;
 using fv = vec<float, SC_VC>;
 
 struct Seq { const void* p; int64_t sn, sl; };                     // [n, length, width] with its strides; channels are contiguous
@@ -57,7 +67,7 @@ __device__ __forceinline__ void decay(fv k, fv sr, fv& l, fv& a, fv& beta) {
             if (l[j] < -0.5f) { a[j] = far; m[j] = far - 1.f; }
         }
 #pragma unroll
-    for (int j = 0; j < SC_VC; ++j) beta[j] = __builtin_amdgcn_sqrtf(-m[j] * (1.f + a[j]));
+    for (int j = 0; j < SC_VC; ++j) beta[j] = __builtin_amdgcn_sqrtf(__builtin_fmaf(-m[j], a[j], -m[j]));
 }
 
 __device__ __forceinline__ fv sigmoid_of(fv v) {
@@ -97,72 +107,54 @@ __device__ __forceinline__ fv rates(const float* __restrict__ lam, float sharpne
     return k;
 }
 
-struct Totals { fv a[2][SC_WAVES][SC_LANES], h[2][SC_WAVES][SC_LANES]; };   // two tiles in turn, so that one barrier a tile is enough
+// where a lane is: channels [c, + SC_VC), steps [t, + STEPS) of a tile, which is run `run` of it
+template <typename S> struct Lane {
+    int cl = threadIdx.x & (SC_LANES - 1), run = threadIdx.x / SC_LANES, group = run & (SC_GROUPS - 1);
+    int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), c = blockIdx.x * SC_CH + SC_VC * cl, t = run * S::STEPS;
+    __device__ __forceinline__ Lane() {}
+};
 
-// Compose the runs of a tile, first step first.  In: this lane's composition (A, H) and the state before the tile.  Out: the state before this
-// lane's steps; `carry` becomes the state after the tile, and `through` (where given) takes the tile's product of decays.
-__device__ __forceinline__ fv join_forward(Totals& tot, int buf, int wave, int group, int cl, fv A, fv H, fv& carry, fv* through = nullptr) {
+template <typename S> struct Totals { fv a[2][S::WAVES][SC_LANES], h[2][S::WAVES][SC_LANES]; };      // two tiles in turn: one barrier a tile is enough
+
+// The compositions of a tile's runs, in the order DIR (1: from the first run, -1: from the last).  put: this lane's (A, H), a barrier, get: the
+// composition (pa, ph) of the runs before this lane's and (ta, th) of the whole tile.
+template <typename S, int DIR>
+struct Join {
+    fv pa, ph, ta, th;
+    static __device__ __forceinline__ fv before(fv v, int groups) { return DIR > 0 ? shuffle_up(v, SC_LANES * groups) : shuffle_down(v, SC_LANES * groups); }
+    __device__ __forceinline__ void put(Totals<S>& tot, int buf, const Lane<S>& at, fv A, fv H) {
+        const int place = DIR > 0 ? at.group : SC_GROUPS - 1 - at.group;
 #pragma unroll
-    for (int by = 1; by < SC_GROUPS; by <<= 1) {
-        const fv pa = shuffle_up(A, SC_LANES * by), ph = shuffle_up(H, SC_LANES * by);
-        if (group >= by) { H = A * ph + H; A = A * pa; }
+        for (int by = 1; by < SC_GROUPS; by <<= 1) {
+            const fv a = before(A, by), h = before(H, by);
+            if (place >= by) { H = A * h + H; A = A * a; }
+        }
+        if (place == SC_GROUPS - 1) { tot.a[buf][at.wave][at.cl] = A; tot.h[buf][at.wave][at.cl] = H; }
+        pa = before(A, 1), ph = before(H, 1);
+        if (place == 0) { pa = fv(1.f); ph = fv(0.f); }
     }
-    if (group == SC_GROUPS - 1) { tot.a[buf][wave][cl] = A; tot.h[buf][wave][cl] = H; }
-    const fv pa = shuffle_up(A, SC_LANES), ph = shuffle_up(H, SC_LANES);
-    __syncthreads();
-    fv at = carry;
+    __device__ __forceinline__ void get(const Totals<S>& tot, int buf, const Lane<S>& at) {
+        ta = fv(1.f), th = fv(0.f);
+        fv wa = ta, wh = th;
 #pragma unroll 4
-    for (int w = 0; w < SC_WAVES; ++w) {
-        const fv a = tot.a[buf][w][cl], h = tot.h[buf][w][cl];
-        if (w == wave) at = carry;
-        carry = a * carry + h;
-        if (through != nullptr) *through = a * *through;
+        for (int q = 0; q < S::WAVES; ++q) {
+            const int w = DIR > 0 ? q : S::WAVES - 1 - q;
+            if (w == at.wave) { wa = ta; wh = th; }
+            const fv a = tot.a[buf][w][at.cl], h = tot.h[buf][w][at.cl];
+            th = a * th + h;
+            ta = a * ta;
+        }
+        ph = pa * wh + ph;
+        pa = pa * wa;
     }
-    return group == 0 ? at : pa * at + ph;
-}
+};
 
-// the same from the last step to the first, of the recurrence C_t = a_t (C_(t+1) + g_t): returns the C of the step behind this lane's last.  The
-// barrier is the caller's, between the two halves.
-__device__ __forceinline__ void join_backward_put(Totals& tot, int buf, int wave, int group, int cl, fv& A, fv& C, fv& na, fv& nc) {
-#pragma unroll
-    for (int by = 1; by < SC_GROUPS; by <<= 1) {
-        const fv a = shuffle_down(A, SC_LANES * by), c = shuffle_down(C, SC_LANES * by);
-        if (group + by < SC_GROUPS) { C = A * c + C; A = A * a; }
-    }
-    if (group == 0) { tot.a[buf][wave][cl] = A; tot.h[buf][wave][cl] = C; }
-    na = shuffle_down(A, SC_LANES), nc = shuffle_down(C, SC_LANES);
-}
-__device__ __forceinline__ fv join_backward_get(const Totals& tot, int buf, int wave, int group, int cl, fv na, fv nc, fv& carry, fv* through = nullptr) {
-    fv at = carry;
-#pragma unroll 4
-    for (int w = SC_WAVES - 1; w >= 0; --w) {
-        const fv a = tot.a[buf][w][cl], c = tot.h[buf][w][cl];
-        if (w == wave) at = carry;
-        carry = a * carry + c;
-        if (through != nullptr) *through = a * *through;
-    }
-    return group == SC_GROUPS - 1 ? at : na * at + nc;
-}
-
-// `carry` through the compositions of `count` chunks from chunk `first` on, in the direction DIR: the SC_RUNS groups of lanes take a run of them each
-template <bool FULL, int DIR>
-__device__ __forceinline__ void join_chunks(Totals& tot, const float* __restrict__ sums, int first, int count, int wave, int group, int tg, int cl, int c,
-                                            int width, fv& carry) {
-    fv A(1.f), H(0.f);
-    const int run = (count + SC_RUNS - 1) / SC_RUNS, end = min(count, (tg + 1) * run);
-#pragma unroll 4
-    for (int q = tg * run; q < end; ++q) {
-        const float* s = sums + (int64_t)(first + DIR * q) * 2 * width;
-        const fv a = load<float, SC_VC, FULL>(s, c, width), h = load<float, SC_VC, FULL>(s + width, c, width);
-        H = a * H + h;
-        A = A * a;
-    }
-    join_forward(tot, 0, wave, group, cl, A, H, carry);
-    __syncthreads();                                                   // the tiles use the same buffers
-}
+// Widths.  Two channels are one load each way: in a row of odd width the last lane loads the last two and takes the second (1 x 10007 x 301 fp16, forward +
+// backward: 110 us with an element a load, 70 so, in chunks of two tiles).
+enum Width { EVEN, ODD, SINGLE };
 
 // N inputs of a sequence, tile by tile: scalar pointers to the tile's head, 32-bit lane offsets into it.
-template <typename T, int N, bool FULL>
+template <typename T, int N, Width W>
 struct Rows {
     const T* head[N];
     int64_t tile[N];                                                   // elements between tiles
@@ -171,7 +163,7 @@ struct Rows {
         tile[q] = SC_TILE * s.sl;
         head[q] = (const T*)s.p + n * s.sn + first_tile * tile[q];
         step[q] = (uint32_t)(s.sl * (int)sizeof(T));
-        idle[q] = (uint32_t)(min(c, width - (FULL ? SC_VC : 1)) * (int)sizeof(T));       // a lane behind the row reads the row's end
+        idle[q] = (uint32_t)(min(c, width - (W == SINGLE ? 1 : SC_VC)) * (int)sizeof(T));       // a lane behind the row reads the row's end
         at[q] = (uint32_t)t * step[q] + idle[q];
     }
     __device__ __forceinline__ void move(int tiles) {
@@ -182,42 +174,73 @@ struct Rows {
 
 // A lane's steps of N inputs as they lie in memory.  Every load is issued, without a branch between them (the compiler then knows how many are in
 // flight, and a tile's wait leaves the next tile's loads alone); what is not live reads the tile's head row again, which costs no traffic.
-template <typename T, int N, bool FULL>
+template <typename T, int N, int STEPS, Width W>
 struct Steps {
-    vec<T, SC_VC> v[N][SC_STEPS];
-    uint32_t live;                                                     // bit s: step s exists and is not masked
+    vec<T, SC_VC> v[N][STEPS];
+    uint32_t live;                                                     // bit s: step s exists and is not masked (looked at where !whole only)
+    bool whole;                                                        // every step of the tile is live
+    bool second;                                                       // (ODD) of what was loaded, only the second is a channel of this lane
+    static __device__ __forceinline__ void one(vec<T, SC_VC>& to, const char* p) { __builtin_memcpy(&to, p, (W == SINGLE ? 1 : SC_VC) * sizeof(T)); }
     // t: this lane's first step in the tile, left: steps from the tile's head to the end (at least 1), mask: of the tile's head
-    __device__ __forceinline__ void fetch(const Rows<T, N, FULL>& rows, const uint8_t* __restrict__ mask, int t, int left, int c, int width) {
+    __device__ __forceinline__ void fetch(const Rows<T, N, W>& rows, const uint8_t* __restrict__ mask, int t, int left, int c, int width) {
+        second = c + 1 == width;
+        if (mask == nullptr && left >= SC_TILE) {                      // all live: one lane offset an input, the steps in the scalar address
+            whole = true;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                for (int q = 0; q < N; ++q) one(v[q][s], reinterpret_cast<const char*>(rows.head[q]) + s * (uint64_t)rows.step[q] + rows.at[q]);
+            return;
+        }
         live = 0;
+        whole = false;
 #pragma unroll
-        for (int s = 0; s < SC_STEPS; ++s) live |= (t + s < left ? 1u : 0u) << s;
+        for (int s = 0; s < STEPS; ++s) live |= (t + s < left ? 1u : 0u) << s;
         if (mask != nullptr) {
-            uint8_t m[SC_STEPS];
+            uint8_t m[STEPS];
 #pragma unroll
-            for (int s = 0; s < SC_STEPS; ++s) m[s] = mask[(uint32_t)min(t + s, left - 1)];
+            for (int s = 0; s < STEPS; ++s) m[s] = mask[(uint32_t)min(t + s, left - 1)];
 #pragma unroll
-            for (int s = 0; s < SC_STEPS; ++s) live &= ~((m[s] == 0 ? 1u : 0u) << s);
+            for (int s = 0; s < STEPS; ++s) live &= ~((m[s] == 0 ? 1u : 0u) << s);
         }
 #pragma unroll
-        for (int s = 0; s < SC_STEPS; ++s)
+        for (int s = 0; s < STEPS; ++s)
 #pragma unroll
             for (int q = 0; q < N; ++q) {
                 const uint32_t at = live >> s & 1u ? rows.at[q] + s * rows.step[q] : rows.idle[q];
-                const char* p = reinterpret_cast<const char*>(rows.head[q]) + at;
-                if constexpr (FULL) __builtin_memcpy(&v[q][s], p, sizeof(v[q][s]));
-                else
-#pragma unroll
-                    for (int k = 0; k < SC_VC; ++k) v[q][s][k] = *reinterpret_cast<const T*>(p + (c + k < width ? k * (int)sizeof(T) : 0));
+                one(v[q][s], reinterpret_cast<const char*>(rows.head[q]) + at);
             }
     }
     __device__ __forceinline__ fv at(int q, int s) const { return __builtin_convertvector(v[q][s], fv); }
+    // A step that is not live: the recurrence gate's logit R becomes -inf -- sigmoid 0, decay 1, beta 0 exactly -- and the other inputs 0, so that
+    // nothing after this asks again whether a step is live, but for what is written
+    template <int R>
+    __device__ __forceinline__ void clean() {
+        if constexpr (W == ODD)
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                for (int q = 0; q < N; ++q) v[q][s][0] = second ? v[q][s][1] : v[q][s][0];
+        if (whole) return;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const bool on = live >> s & 1u;
+#pragma unroll
+            for (int q = 0; q < N; ++q)
+#pragma unroll
+                for (int k = 0; k < SC_VC; ++k) v[q][s][k] = on ? v[q][s][k] : (T)(q == R ? -INFINITY : 0.f);
+        }
+    }
+    __device__ __forceinline__ fv kept(int s, fv f) const {            // what is written, or summed over steps
+        return whole || (live >> s & 1u) ? f : fv(0.f);
+    }
     // hides from the compiler that the values are still the same: what is cheap to form from them is formed again, not kept in registers
     __device__ __forceinline__ void renew() {
         using Bits = typename std::conditional<SC_VC * sizeof(T) == 4, uint32_t, uint64_t>::type;
 #pragma unroll
         for (int q = 0; q < N; ++q)
 #pragma unroll
-            for (int s = 0; s < SC_STEPS; ++s) {
+            for (int s = 0; s < STEPS; ++s) {
                 Bits b = __builtin_bit_cast(Bits, v[q][s]);
                 asm volatile("" : "+v"(b));
                 v[q][s] = __builtin_bit_cast(decltype(v[q][s] + v[q][s]), b);
@@ -225,246 +248,336 @@ struct Steps {
     }
 };
 
-constexpr int ONE_TILE = 0, TILES = 1, SUMMARY = 2;                    // sequences of one tile need no next one fetched ahead
+// A sequence's chunks of tiles, each with its composition [2, width] in `sums`: the state that enters after `count` chunks from `first` on, in the order
+// DIR, if `edge` enters the first.  The runs of a workgroup share the chunks out.
+template <bool FULL, int DIR, typename S>
+__device__ __forceinline__ fv entering(Totals<S>& tot, const float* __restrict__ sums, int first, int count, fv edge, const Lane<S>& at, int width) {
+    fv A(1.f), H(0.f);
+    const int each = (count + S::RUNS - 1) / S::RUNS, end = min(count, (at.run + 1) * each);
+#pragma unroll 4
+    for (int q = at.run * each; q < end; ++q) {
+        const float* s = sums + (int64_t)(first + DIR * q) * 2 * width;
+        const fv a = load<float, SC_VC, FULL>(s, at.c, width), h = load<float, SC_VC, FULL>(s + width, at.c, width);
+        H = a * H + h;
+        A = A * a;
+    }
+    Join<S, 1> j;
+    j.put(tot, 1, at, A, H);                                           // (the first tile uses the other half)
+    __syncthreads();
+    j.get(tot, 1, at);
+    return j.ta * edge + j.th;
+}
 
 // the byte offset of step t, channel c in a tile of a contiguous output
 template <typename T>
 __device__ __forceinline__ uint32_t lane_offset(int t, int width, int c) { return (uint32_t)((t * width + c) * (int)sizeof(T)); }
 
-// a and b of a lane's steps; a step that is not live is a = 1, b = 0 whatever was read for it
-template <bool NEAR, typename In>
-__device__ __forceinline__ void gates_forward(const In& in, fv k, fv (&a)[SC_STEPS], fv (&b)[SC_STEPS]) {
+// a and b of a lane's steps
+template <bool NEAR, int STEPS, typename In>
+__device__ __forceinline__ void gates_forward(const In& in, fv k, fv (&a)[STEPS], fv (&b)[STEPS]) {
 #pragma unroll
-    for (int s = 0; s < SC_STEPS; ++s) {
+    for (int s = 0; s < STEPS; ++s) {
         fv l, beta;
         decay<NEAR>(k, sigmoid_of(in.at(1, s)), l, a[s], beta);
         b[s] = beta * (sigmoid_of(in.at(2, s)) * in.at(0, s));
-        const bool live = in.live >> s & 1u;
-#pragma unroll
-        for (int j = 0; j < SC_VC; ++j) { a[s][j] = live ? a[s][j] : 1.f; b[s][j] = live ? b[s][j] : 0.f; }
     }
 }
 
-// One workgroup: channels [64 blockIdx.x, + 64) of sequence blockIdx.y, tiles [chunk * per, + per).  The next tile's loads are in flight
-// while a tile is computed.  SUMMARY: only the chunk's composition goes to `sums` [n, chunks, 2, width].
-template <typename T, bool FULL, int MODE>
-__global__ __launch_bounds__(SC_THREADS, 4) void scan_fwd_kernel(Seq x, Seq r, Seq i, const float* __restrict__ lam, float sharpness,
-                                                                 const uint8_t* __restrict__ mask, int64_t mask_sn, const float* __restrict__ state,
-                                                                 T* __restrict__ h, float* __restrict__ last, float* __restrict__ tiles,
-                                                                 float* __restrict__ sums, int length, int width, int chunks, int per) {
-    __shared__ Totals tot;
-    const int cl = threadIdx.x & (SC_LANES - 1), tg = threadIdx.x / SC_LANES, group = tg & (SC_GROUPS - 1);
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int c = blockIdx.x * SC_CH + SC_VC * cl, chunk = blockIdx.z, t = tg * SC_STEPS;
+// a, b of a lane's steps and their composition; false if the wave has none that is live
+template <typename In, int STEPS>
+__device__ __forceinline__ bool compose(In& in, bool near, fv k, fv (&a)[STEPS], fv (&b)[STEPS], fv& A, fv& H) {
+    A = fv(1.f), H = fv(0.f);
+    if (!in.whole && !__any(in.live != 0)) return false;               // (a wave past the end of its sequence has nothing to do)
+    in.template clean<1>();
+    if (near) gates_forward<true>(in, k, a, b);
+    else gates_forward<false>(in, k, a, b);
+    A = a[0], H = b[0];
+#pragma unroll
+    for (int s = 1; s < STEPS; ++s) {
+        H = a[s] * H + b[s];
+        A = A * a[s];
+    }
+    return true;
+}
+
+// h of a lane's steps from the state before them
+template <typename T, bool FULL, int STEPS>
+__device__ __forceinline__ void replay(bool whole, uint32_t live, bool some, const fv (&a)[STEPS], const fv (&b)[STEPS], fv now, T* head, uint32_t at_h, int t,
+                                       int left, int c, int width) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        if (some) now = a[s] * now + b[s];
+        if (whole || t + s < left) store_at<T, SC_VC, FULL>(head + s * width, at_h, c, width, whole || (live >> s & 1u) ? now : fv(0.f));
+    }
+}
+
+// Workgroup: channels [64 blockIdx.x, + 64) of sequence blockIdx.y, tiles [per blockIdx.z, + per) one after the other; the next tile's loads are in flight
+// while a tile is computed.  ONE: sequences of one tile, which need no registers for a next one.  SUM: only the chunk's composition, to `sums`
+// [n, chunks, 2, width]; chunks after the first start from those.
+enum class Pass { ONE, TILES, SUM };
+template <typename T, Width W, Pass PASS>
+__global__ __launch_bounds__(Fwd::THREADS, 4) void scan_fwd_kernel(Seq x, Seq r, Seq i, const float* __restrict__ lam, float sharpness,
+                                                                   const uint8_t* __restrict__ mask, int64_t mask_sn, const float* __restrict__ state,
+                                                                   T* __restrict__ h, float* __restrict__ last, float* __restrict__ tiles,
+                                                                   float* __restrict__ sums, int length, int width, int per) {
+    using S = Fwd;
+    constexpr bool FULL = W == EVEN;
+    __shared__ Totals<S> tot;
+    const Lane<S> at;
     const int64_t n = blockIdx.y;
-    const int n_tiles = (length + SC_TILE - 1) / SC_TILE, t_begin = chunk * per, t_end = min(n_tiles, t_begin + per);
-    if (t_begin >= t_end) return;
-    Rows<T, 3, FULL> rows;
-    rows.set(0, x, n, t_begin, t, c, width);
-    rows.set(1, r, n, t_begin, t, c, width);
-    rows.set(2, i, n, t_begin, t, c, width);
-    const uint8_t* m = mask != nullptr ? mask + n * mask_sn + t_begin * SC_TILE : nullptr;
-    int left = length - t_begin * SC_TILE;
-    Steps<T, 3, FULL> in, ahead;
-    in.fetch(rows, m, t, left, c, width);
-    const fv k = rates<FULL>(lam, sharpness, c, width), zero(0.f);
+    const int c = at.c, t = at.t, n_tiles = PASS == Pass::ONE ? 1 : (length + SC_TILE - 1) / SC_TILE;
+    const int first = PASS == Pass::ONE ? 0 : blockIdx.z * per, end = min(n_tiles, first + per);        // (every chunk has a tile)
+    Rows<T, 3, W> rows;
+    rows.set(0, x, n, first, t, c, width);
+    rows.set(1, r, n, first, t, c, width);
+    rows.set(2, i, n, first, t, c, width);
+    if (mask != nullptr) mask += n * mask_sn;
+    Steps<T, 3, S::STEPS, W> in, ahead;
+    in.fetch(rows, mask != nullptr ? mask + (int64_t)first * SC_TILE : nullptr, t, length - first * SC_TILE, c, width);
+    const fv k = rates<FULL>(lam, sharpness, c, width);
     const bool near = all_near(k);
     const uint32_t at_h = lane_offset<T>(t, width, c);
     fv carry(0.f), through(1.f);
-    if constexpr (MODE != SUMMARY) {
-        if (state != nullptr) carry = load<float, SC_VC, FULL>(state + n * width, c, width);
-        if (MODE == TILES && chunk > 0) join_chunks<FULL, 1>(tot, sums + n * chunks * 2 * width, 0, chunk, wave, group, tg, cl, c, width, carry);
-    }
-    for (int tile = t_begin; tile < t_end; ++tile, left -= SC_TILE) {
-        if (MODE != ONE_TILE && tile + 1 < t_end) {
+    if (PASS != Pass::SUM && state != nullptr) carry = load<float, SC_VC, FULL>(state + n * width, c, width);
+    if (PASS == Pass::TILES && blockIdx.z > 0) carry = entering<FULL, 1>(tot, sums + n * gridDim.z * 2 * width, 0, blockIdx.z, carry, at, width);
+    for (int tile = first, buf = 0;; ++tile, buf ^= 1) {
+        const int left = length - tile * SC_TILE;
+        if (PASS != Pass::ONE && tile + 1 < end) {
             rows.move(1);
-            if (m != nullptr) m += SC_TILE;
-            ahead.fetch(rows, m, t, left - SC_TILE, c, width);
+            ahead.fetch(rows, mask != nullptr ? mask + (int64_t)(tile + 1) * SC_TILE : nullptr, t, left - SC_TILE, c, width);
         }
-        fv a[SC_STEPS], b[SC_STEPS], A(1.f), H(0.f);
-        if (__any(in.live != 0)) {
-            if (near) gates_forward<true>(in, k, a, b);
-            else gates_forward<false>(in, k, a, b);
-#pragma unroll
-            for (int s = 0; s < SC_STEPS; ++s) {
-                H = a[s] * H + b[s];
-                A = A * a[s];
-            }
-        }
-        if constexpr (MODE == SUMMARY) join_forward(tot, tile & 1, wave, group, cl, A, H, carry, &through);
+        fv a[S::STEPS], b[S::STEPS], A, H;
+        const bool some = compose(in, near, k, a, b, A, H);
+        Join<S, 1> j;
+        j.put(tot, buf, at, A, H);
+        __syncthreads();
+        j.get(tot, buf, at);
+        if constexpr (PASS == Pass::SUM) through = j.ta * through;
         else {
-            if (tiles != nullptr && tg == 0) store<float, SC_VC, FULL>(tiles + (n * n_tiles + tile) * width, c, width, carry);
-            fv now = join_forward(tot, tile & 1, wave, group, cl, A, H, carry);
-            T* head = h + (n * length + (int64_t)tile * SC_TILE) * width;
-#pragma unroll
-            for (int s = 0; s < SC_STEPS; ++s) {
-                fv out = zero;
-                if (in.live >> s & 1u) out = now = a[s] * now + b[s];
-                if (t + s < left) store_at<T, SC_VC, FULL>(head + s * width, at_h, c, width, out);
-            }
+            if (tiles != nullptr && at.run == 0) store<float, SC_VC, FULL>(tiles + (n * n_tiles + tile) * width, c, width, carry);
+            replay<T, FULL>(in.whole, in.live, some, a, b, j.pa * carry + j.ph, h + (n * length + (int64_t)tile * SC_TILE) * width, at_h, t, left, c, width);
         }
-        if constexpr (MODE != ONE_TILE) in = ahead;
+        carry = j.ta * carry + j.th;
+        if (PASS == Pass::ONE || tile + 1 == end) break;
+        in = ahead;
     }
-    if (tg == 0) {
-        if constexpr (MODE == SUMMARY) {
-            float* s = sums + ((n * chunks + chunk) * 2) * width;
-            store<float, SC_VC, FULL>(s, c, width, through);
-            store<float, SC_VC, FULL>(s + width, c, width, carry);
-        } else if (t_end == n_tiles) store<float, SC_VC, FULL>(last + n * width, c, width, carry);
-    }
+    if (at.run != 0) return;
+    if constexpr (PASS == Pass::SUM) {
+        float* s = sums + (n * gridDim.z + blockIdx.z) * 2 * width;
+        store<float, SC_VC, FULL>(s, c, width, through);
+        store<float, SC_VC, FULL>(s + width, c, width, carry);
+    } else if (end == n_tiles) store<float, SC_VC, FULL>(last + n * width, c, width, carry);
 }
 
-template <bool NEAR, bool ALL, typename In>
-__device__ __forceinline__ void gates_backward(const In& in, fv k, fv (&sr)[SC_STEPS], fv (&si)[SC_STEPS], fv (&a)[SC_STEPS], fv (&beta)[SC_STEPS]) {
+template <bool NEAR, int STEPS, typename In>
+__device__ __forceinline__ void gates_backward(const In& in, fv k, fv (&sr)[STEPS], fv (&si)[STEPS], fv (&a)[STEPS], fv (&beta)[STEPS]) {
 #pragma unroll
-    for (int s = 0; s < SC_STEPS; ++s) {
+    for (int s = 0; s < STEPS; ++s) {
         fv l;
         sr[s] = sigmoid_of(in.at(0, s));
         decay<NEAR>(k, sr[s], l, a[s], beta[s]);
-        if constexpr (ALL) si[s] = sigmoid_of(in.at(3, s));
-        const bool live = in.live >> s & 1u;
-#pragma unroll
-        for (int j = 0; j < SC_VC; ++j) a[s][j] = live ? a[s][j] : 1.f;
+        si[s] = sigmoid_of(in.at(3, s));
     }
 }
 
-// Backward.  C_t = a_t G_t is what step t hands to step t - 1: C_t = a_t (C_(t+1) + dh_t), G_t = dh_t + C_(t+1).
-//   SUMMARY: the chunk's composition of the C recurrence (reads r and dh only)
-template <typename T, bool FULL, int MODE>
-__global__ __launch_bounds__(SC_THREADS, 4) void scan_bwd_kernel(Seq x, Seq r, Seq i, Seq gh, const float* __restrict__ lam, float sharpness,
-                                                                 const uint8_t* __restrict__ mask, int64_t mask_sn, const float* __restrict__ tiles,
-                                                                 const float* __restrict__ glast, T* __restrict__ dx, T* __restrict__ dr,
-                                                                 T* __restrict__ di, float* __restrict__ dstate, float* __restrict__ qsum,
-                                                                 float* __restrict__ sums, int seqs, int length, int width, int chunks, int per) {
-    __shared__ Totals tot, fwd;
-    __shared__ fv fold[SC_RUNS][SC_LANES];
-    constexpr int N = MODE == SUMMARY ? 2 : 4;
-    constexpr bool AHEAD = MODE == SUMMARY;                            // four inputs leave no registers for a second tile
-    const int cl = threadIdx.x & (SC_LANES - 1), tg = threadIdx.x / SC_LANES, group = tg & (SC_GROUPS - 1);
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int c = blockIdx.x * SC_CH + SC_VC * cl, chunk = blockIdx.z, t = tg * SC_STEPS;
-    const int n_tiles = (length + SC_TILE - 1) / SC_TILE, t_begin = chunk * per, t_end = min(n_tiles, t_begin + per);
-    const fv k = rates<FULL>(lam, sharpness, c, width), zero(0.f);
+// Backward.  C_t = a_t G_t is what step t hands to step t - 1: C_t = a_t (C_(t+1) + dh_t), G_t = dh_t + C_(t+1).  Tiles from the last to the first.
+// inputs of `in`: 0 r, 1 dh, 2 x, 3 i
+template <typename In, int STEPS>
+__device__ __forceinline__ bool compose_both(In& in, bool near, fv k, fv (&sr)[STEPS], fv (&si)[STEPS], fv (&a)[STEPS], fv (&beta)[STEPS], fv& A, fv& H,
+                                             fv& C) {
+    A = fv(1.f), H = fv(0.f), C = fv(0.f);
+    if (!in.whole && !__any(in.live != 0)) return false;
+    in.template clean<0>();
+    if (near) gates_backward<true>(in, k, sr, si, a, beta);
+    else gates_backward<false>(in, k, sr, si, a, beta);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        H = a[s] * H + beta[s] * (si[s] * in.at(2, s));
+        A = A * a[s];
+    }
+#pragma unroll
+    for (int s = STEPS - 1; s >= 0; --s) C = a[s] * (C + in.at(1, s));
+    return true;
+}
+
+template <typename T> struct Grads { T *dx, *dr, *di; };
+template <typename T> Grads<T> grads(void* dx, void* dr, void* di) { return {(T*)dx, (T*)dr, (T*)di}; }
+
+// the gradients of a lane's steps: `now` the state before them, `back` the C of the step behind them
+template <typename T, bool FULL, typename In, int STEPS>
+__device__ __forceinline__ void gradients(In& in, bool some, fv k, fv (&sr)[STEPS], fv (&si)[STEPS], fv (&a)[STEPS], fv (&beta)[STEPS], fv now, fv back,
+                                          fv& q_all, Grads<T> d, int64_t row, uint32_t at_d, int t, int left, int c, int width) {
+    if (some) {
+        in.renew();
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) asm volatile("" : "+v"(sr[s]), "+v"(si[s]), "+v"(beta[s]));
+        fv before[STEPS];
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            before[s] = now;
+            now = a[s] * now + beta[s] * (si[s] * in.at(2, s));
+        }
+#pragma unroll
+        for (int s = STEPS - 1; s >= 0; --s) {
+            const fv G = in.at(1, s) + back, xs = in.at(2, s), du = G * beta[s], u = si[s] * xs, l = k * sr[s];
+            back = a[s] * G;
+            fv lb;                                                         // l / beta tends to 0 with l (as -sqrt(-l / 2)): where beta has become 0, so has l
+#pragma unroll
+            for (int q = 0; q < SC_VC; ++q) lb[q] = beta[s][q] > 0.f ? l[q] * __builtin_amdgcn_rcpf(beta[s][q]) : 0.f;
+            const fv q = in.kept(s, back * (before[s] * l - u * a[s] * lb));
+            q_all += q;
+            if (!in.whole && t + s >= left) continue;
+            store_at<T, SC_VC, FULL>(d.dx + row + s * width, at_d, c, width, in.kept(s, du * si[s]));
+            store_at<T, SC_VC, FULL>(d.dr + row + s * width, at_d, c, width, in.kept(s, q * (1.f - sr[s])));
+            store_at<T, SC_VC, FULL>(d.di + row + s * width, at_d, c, width, in.kept(s, du * u * (1.f - si[s])));
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            if (t + s >= left) continue;
+            store_at<T, SC_VC, FULL>(d.dx + row + s * width, at_d, c, width, fv(0.f));
+            store_at<T, SC_VC, FULL>(d.dr + row + s * width, at_d, c, width, fv(0.f));
+            store_at<T, SC_VC, FULL>(d.di + row + s * width, at_d, c, width, fv(0.f));
+        }
+    }
+}
+
+// a part of sum q, its lanes in a fixed order
+template <bool FULL, typename S>
+__device__ __forceinline__ void fold_q(fv (&fold)[S::RUNS][SC_LANES], fv q_all, float* qsum, const Lane<S>& at, int width) {
+    fold[at.run][at.cl] = q_all;
+    __syncthreads();
+    if (at.run != 0) return;
+    fv s = fold[0][at.cl];
+#pragma unroll
+    for (int w = 1; w < S::RUNS; ++w) s += fold[w][at.cl];
+    store<float, SC_VC, FULL>(qsum, at.c, width, s);
+}
+
+// The composition of a chunk's C recurrence, for few sequences (r and dh alone are read), to `sums` [n, chunks, 2, width]
+template <typename T, Width W>
+__global__ __launch_bounds__(Bwd::THREADS, 2) void scan_bwd_sum_kernel(Seq r, Seq gh, const float* __restrict__ lam, float sharpness,
+                                                                       const uint8_t* __restrict__ mask, int64_t mask_sn, float* __restrict__ sums,
+                                                                       int length, int width, int per) {
+    using S = Bwd;
+    constexpr bool FULL = W == EVEN;
+    __shared__ Totals<S> tot;
+    const Lane<S> at;
+    const int64_t n = blockIdx.y;
+    const int c = at.c, t = at.t, n_tiles = (length + SC_TILE - 1) / SC_TILE, first = blockIdx.z * per, end = min(n_tiles, first + per);
+    Rows<T, 2, W> rows;
+    rows.set(0, r, n, end - 1, t, c, width);
+    rows.set(1, gh, n, end - 1, t, c, width);
+    if (mask != nullptr) mask += n * mask_sn;
+    Steps<T, 2, S::STEPS, W> in, ahead;
+    in.fetch(rows, mask != nullptr ? mask + (int64_t)(end - 1) * SC_TILE : nullptr, t, length - (end - 1) * SC_TILE, c, width);
+    const fv k = rates<FULL>(lam, sharpness, c, width);
+    const bool near = all_near(k);
+    fv carry(0.f), through(1.f);
+    for (int tile = end - 1, buf = 0;; --tile, buf ^= 1) {
+        if (tile > first) {
+            rows.move(-1);
+            ahead.fetch(rows, mask != nullptr ? mask + (int64_t)(tile - 1) * SC_TILE : nullptr, t, length - (tile - 1) * SC_TILE, c, width);
+        }
+        fv A(1.f), C(0.f);
+        in.template clean<0>();
+#pragma unroll
+        for (int s = S::STEPS - 1; s >= 0; --s) {
+            fv l, a, beta;
+            if (near) decay<true>(k, sigmoid_of(in.at(0, s)), l, a, beta);
+            else decay<false>(k, sigmoid_of(in.at(0, s)), l, a, beta);
+            C = a * (C + in.at(1, s));
+            A = A * a;
+        }
+        Join<S, -1> j;
+        j.put(tot, buf, at, A, C);
+        __syncthreads();
+        j.get(tot, buf, at);
+        through = j.ta * through;
+        carry = j.ta * carry + j.th;
+        if (tile == first) break;
+        in = ahead;
+    }
+    if (at.run != 0) return;
+    float* s = sums + (n * gridDim.z + blockIdx.z) * 2 * width;
+    store<float, SC_VC, FULL>(s, c, width, through);
+    store<float, SC_VC, FULL>(s + width, c, width, carry);
+}
+
+// Workgroup: channels [64 blockIdx.x, + 64) of sequences blockIdx.y, + gridDim.y, .., tiles [per blockIdx.z, + per) from the last one on
+template <typename T, Width W>
+__global__ __launch_bounds__(Bwd::THREADS, 2) void scan_bwd_kernel(Seq x, Seq r, Seq i, Seq gh, const float* __restrict__ lam, float sharpness,
+                                                                   const uint8_t* __restrict__ mask, int64_t mask_sn, const float* __restrict__ tiles,
+                                                                   const float* __restrict__ glast, Grads<T> d, float* __restrict__ dstate,
+                                                                   float* __restrict__ qsum, const float* __restrict__ sums, int seqs, int length,
+                                                                   int width, int per) {
+    using S = Bwd;
+    constexpr bool FULL = W == EVEN;
+    __shared__ Totals<S> tot, fwd;
+    __shared__ fv fold[S::RUNS][SC_LANES];
+    const Lane<S> at;
+    const int c = at.c, t = at.t, n_tiles = (length + SC_TILE - 1) / SC_TILE, chunks = gridDim.z, first = blockIdx.z * per, end = min(n_tiles, first + per);
+    const fv k = rates<FULL>(lam, sharpness, c, width);
     const bool near = all_near(k);
     const uint32_t at_d = lane_offset<T>(t, width, c);
-    fv q_all(0.f);
-    int buf = 0;
-    for (int64_t n = blockIdx.y; n < seqs && t_begin < t_end; n += gridDim.y) {
-        Rows<T, N, FULL> rows;
-        rows.set(0, r, n, t_end - 1, t, c, width);
-        rows.set(1, gh, n, t_end - 1, t, c, width);
-        if constexpr (MODE != SUMMARY) {
-            rows.set(2, x, n, t_end - 1, t, c, width);
-            rows.set(3, i, n, t_end - 1, t, c, width);
-        }
-        const uint8_t* m = mask != nullptr ? mask + n * mask_sn + (t_end - 1) * SC_TILE : nullptr;
-        int left = length - (t_end - 1) * SC_TILE;
-        Steps<T, N, FULL> in, ahead;
-        in.fetch(rows, m, t, left, c, width);
-        fv carry(0.f), through(1.f);
-        if constexpr (MODE != SUMMARY) {
-            if (glast != nullptr) carry = load<float, SC_VC, FULL>(glast + n * width, c, width);
-            if (MODE == TILES && chunk < chunks - 1)
-                join_chunks<FULL, -1>(tot, sums + n * chunks * 2 * width, chunks - 1, chunks - 1 - chunk, wave, group, tg, cl, c, width, carry);
-        }
-        for (int tile = t_end - 1; tile >= t_begin; --tile, buf ^= 1, left += SC_TILE) {
-            fv head(0.f);
-            if constexpr (MODE != SUMMARY) head = load<float, SC_VC, FULL>(tiles + (n * n_tiles + tile) * width, c, width);
-            if (MODE != ONE_TILE && tile > t_begin) {
-                rows.move(-1);
-                if (m != nullptr) m -= SC_TILE;
-                if constexpr (AHEAD) ahead.fetch(rows, m, t, left + SC_TILE, c, width);
-            }
-            fv sr[SC_STEPS], si[SC_STEPS], a[SC_STEPS], beta[SC_STEPS], A(1.f), H(0.f), C(0.f);
-            if (__any(in.live != 0)) {
-                if (near) gates_backward<true, MODE != SUMMARY>(in, k, sr, si, a, beta);
-                else gates_backward<false, MODE != SUMMARY>(in, k, sr, si, a, beta);
-#pragma unroll
-                for (int s = 0; s < SC_STEPS; ++s) {
-                    if constexpr (MODE != SUMMARY)
-                        if (in.live >> s & 1u) H = a[s] * H + beta[s] * (si[s] * in.at(2, s));
-                    A = A * a[s];
-                }
-#pragma unroll
-                for (int s = SC_STEPS - 1; s >= 0; --s)
-                    if (in.live >> s & 1u) C = a[s] * (C + in.at(1, s));
-            }
-            fv Ar = A, na, nc, now(0.f);
-            join_backward_put(tot, buf, wave, group, cl, Ar, C, na, nc);
-            if constexpr (MODE != SUMMARY) now = join_forward(fwd, buf, wave, group, cl, A, H, head);     // its barrier covers `tot` too
-            else __syncthreads();
-            fv back = join_backward_get(tot, buf, wave, group, cl, na, nc, carry, MODE == SUMMARY ? &through : nullptr);
-            if constexpr (MODE != SUMMARY) {
-                const int64_t row = (n * length + (int64_t)tile * SC_TILE) * width;
-                in.renew();
-#pragma unroll
-                for (int s = 0; s < SC_STEPS; ++s) asm volatile("" : "+v"(sr[s]), "+v"(si[s]), "+v"(beta[s]));
-                fv before[SC_STEPS];
-#pragma unroll
-                for (int s = 0; s < SC_STEPS; ++s) {
-                    before[s] = now;
-                    if (in.live >> s & 1u) now = a[s] * now + beta[s] * (si[s] * in.at(2, s));
-                }
-#pragma unroll
-                for (int s = SC_STEPS - 1; s >= 0; --s) {
-                    if (t + s >= left) continue;
-                    fv vx = zero, vr = zero, vi = zero;
-                    if (in.live >> s & 1u) {
-                        const fv G = in.at(1, s) + back, xs = in.at(2, s);
-                        back = a[s] * G;
-#pragma unroll
-                        for (int j = 0; j < SC_VC; ++j) {
-                            const float l = k[j] * sr[s][j], bv = beta[s][j], u = si[s][j] * xs[j];
-                            // l / beta tends to 0 with l (as -sqrt(-l / 2)): where beta has become 0, so has l
-                            const float lb = bv > 0.f ? l * __builtin_amdgcn_rcpf(bv) : 0.f;
-                            const float q = back[j] * (before[s][j] * l - u * a[s][j] * lb), du = G[j] * bv;
-                            q_all[j] += q;
-                            vx[j] = du * si[s][j];
-                            vr[j] = q * (1.f - sr[s][j]);
-                            vi[j] = du * u * (1.f - si[s][j]);
-                        }
-                    }
-                    store_at<T, SC_VC, FULL>(dx + row + s * width, at_d, c, width, vx);
-                    store_at<T, SC_VC, FULL>(dr + row + s * width, at_d, c, width, vr);
-                    store_at<T, SC_VC, FULL>(di + row + s * width, at_d, c, width, vi);
-                }
-            }
-            if constexpr (AHEAD) in = ahead;
-            else if (MODE != ONE_TILE && tile > t_begin) in.fetch(rows, m, t, left + SC_TILE, c, width);
-        }
-        if (tg == 0) {
-            if constexpr (MODE == SUMMARY) {
-                float* s = sums + ((n * chunks + chunk) * 2) * width;
-                store<float, SC_VC, FULL>(s, c, width, through);
-                store<float, SC_VC, FULL>(s + width, c, width, carry);
-            } else if (chunk == 0 && dstate != nullptr) store<float, SC_VC, FULL>(dstate + n * width, c, width, carry);
-        }
-    }
-    if constexpr (MODE != SUMMARY) {                                   // this workgroup's part of sum q, in a fixed order
-        fold[tg][cl] = q_all;
+    fv q_all(0.f), carry(0.f);
+    Rows<T, 4, W> rows;
+    Steps<T, 4, S::STEPS, W> in;
+    int tile = end - 1;
+    int64_t n = blockIdx.y;
+    if (glast != nullptr) carry = load<float, SC_VC, FULL>(glast + n * width, c, width);
+    if (end < n_tiles) carry = entering<FULL, -1>(tot, sums + n * chunks * 2 * width, chunks - 1, chunks - 1 - (int)blockIdx.z, carry, at, width);
+    // (sequences that are cut have a workgroup each, so that what follows takes no second one of them.)  One loop over sequences and tiles: nested, the compiler spills 45 registers
+    for (int buf = 0; n < seqs; buf ^= 1) {
+        const int left = length - tile * SC_TILE;
+        rows.set(0, r, n, tile, t, c, width);
+        rows.set(1, gh, n, tile, t, c, width);
+        rows.set(2, x, n, tile, t, c, width);
+        rows.set(3, i, n, tile, t, c, width);
+        in.fetch(rows, mask != nullptr ? mask + n * mask_sn + (int64_t)tile * SC_TILE : nullptr, t, left, c, width);
+        const fv head = load<float, SC_VC, FULL>(tiles + (n * n_tiles + tile) * width, c, width);
+        fv sr[S::STEPS], si[S::STEPS], a[S::STEPS], beta[S::STEPS], A, H, C;
+        const bool some = compose_both(in, near, k, sr, si, a, beta, A, H, C);
+        Join<S, 1> f;
+        Join<S, -1> j;
+        f.put(fwd, buf, at, A, H);
+        j.put(tot, buf, at, A, C);
         __syncthreads();
-        if (tg == 0) {
-            fv s = fold[0][cl];
-#pragma unroll
-            for (int w = 1; w < SC_RUNS; ++w) s += fold[w][cl];
-            store<float, SC_VC, FULL>(qsum + ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * width, c, width, s);
+        f.get(fwd, buf, at);
+        j.get(tot, buf, at);
+        const fv now = f.pa * head + f.ph, back = j.pa * carry + j.ph;
+        carry = j.ta * carry + j.th;
+        if (tile == 0 && at.run == 0 && dstate != nullptr) store<float, SC_VC, FULL>(dstate + n * width, c, width, carry);
+        gradients<T, FULL>(in, some, k, sr, si, a, beta, now, back, q_all, d, (n * length + (int64_t)tile * SC_TILE) * width, at_d, t, left, c, width);
+        if (--tile < first) {
+            tile = end - 1;
+            n += gridDim.y;
+            carry = fv(0.f);
+            if (glast != nullptr && n < seqs) carry = load<float, SC_VC, FULL>(glast + n * width, c, width);
         }
     }
+    fold_q<FULL>(fold, q_all, qsum + ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * width, at, width);
 }
 
-// dlam = sum q sigmoid(lam) / softplus(lam): `parts` rows of partial sums, 16 columns x 16 row lanes a workgroup, fixed order
-__global__ __launch_bounds__(256) void scan_dlam_kernel(const float* __restrict__ qsum, int parts, const float* __restrict__ lam, float* __restrict__ dlam,
-                                                        int width) {
-    __shared__ float red[16][17];
+// dlam = sum q sigmoid(lam) / softplus(lam): `parts` rows of partial sums, 16 columns x 64 row lanes a workgroup, 8 rows of a lane in flight, in a fixed
+// order (512 x 50 x 256, 512 rows: 16 lanes, one row in flight 8.2 us, this 4.4)
+__global__ __launch_bounds__(1024) void scan_dlam_kernel(const float* __restrict__ qsum, int parts, const float* __restrict__ lam, float* __restrict__ dlam,
+                                                         int width) {
+    __shared__ float red[64][17];
     const int col = threadIdx.x & 15, lane = threadIdx.x >> 4, c = blockIdx.x * 16 + col;
     float s = 0.f;
     if (c < width)
-        for (int p = lane; p < parts; p += 16) s += qsum[(int64_t)p * width + c];
+        for (int p = lane; p < parts; p += 64 * 8) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = p + 64 * u < parts ? qsum[(int64_t)(p + 64 * u) * width + c] : 0.f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
     red[lane][col] = s;
     __syncthreads();
     if (lane == 0 && c < width) {
-#pragma unroll
-        for (int w = 1; w < 16; ++w) s += red[w][col];
+        for (int w = 1; w < 64; ++w) s += red[w][col];
         const float v = lam[c], sp = softplus(v);
         // sigmoid / softplus -> 1 - e^lam / 2 for lam -> -inf, where both underflow together
         dlam[c] = s * (v < -15.f ? 1.f : 1.f / ((1.f + expf(-v)) * sp));
@@ -496,21 +609,26 @@ __global__ __launch_bounds__(256) void scan_step_kernel(Seq x, Seq r, Seq i, con
 
 struct ScanPlan { int slices, tiles, chunks, per, rows; };
 
-// chunks of a sequence and workgroup rows of the backward pass: one workgroup a (sequence, 64 channels) fills the 256 CUs from about 512
-// workgroups on; below that long sequences are cut until about 1024 are in flight, at least 2 tiles each
+// One workgroup a (sequence, 64 channels) streams as fast as memory gives from about 192 of them on: 256 workgroups, 64 x 2048 x 256 fp32, 109 us forward
+// and 217 backward against 196 and 289 cut into chunks, which read their inputs twice.  Below that sequences of 4 tiles and more are cut until about
+// CUT_TO workgroups are in flight, a tile each at least.  Forward + backward (us) for 512 / 768 / 1024: 2 x 32768 x 768 bf16 430 / 432 / 442,
+// 8 x 4096 x 768 bf16 250 / 224 / 225; at least 1 / 2 / 4 tiles: 1 x 10007 x 301 fp16 62 / 70 / 78, 1 x 2048 x 256 fp32 26 / 34 / 51.  (A single pass
+// over the chunks, each waiting for the one before it, was no faster, 184 + 284 us for the first: what a tile waits for the words of others costs more
+// than its second reading.)
+constexpr int CUT_BELOW = 192, CUT_TO = 768;
 static ScanPlan scan_plan(int n, int length, int width) {
     ScanPlan p;
     p.slices = (width + SC_CH - 1) / SC_CH;
     p.tiles = (length + SC_TILE - 1) / SC_TILE;
     const int64_t wgs = (int64_t)n * p.slices;
     p.chunks = 1;
-    if (wgs < 512 && p.tiles >= 4) {
-        const int64_t want = (1024 + wgs - 1) / wgs;
-        p.chunks = (int)(want < p.tiles / 2 ? want : p.tiles / 2);
+    if (wgs < CUT_BELOW && p.tiles >= 4) {
+        const int64_t want = (CUT_TO + wgs - 1) / wgs;
+        p.chunks = (int)(want < p.tiles ? want : p.tiles);
     }
     p.per = p.tiles > 0 ? (p.tiles + p.chunks - 1) / p.chunks : 1;
-    p.chunks = p.tiles > 0 ? (p.tiles + p.per - 1) / p.per : 1;
-    const int cap = 2048 / p.slices > 0 ? 2048 / p.slices : 1;         // partial rows of sum q
+    p.chunks = p.tiles > 0 ? (p.tiles + p.per - 1) / p.per : 1;        // (none is empty)
+    const int cap = 2048 / p.slices > 0 ? 2048 / p.slices : 1;         // backward: workgroups that take sequences one after the other
     p.rows = n < cap ? n : cap;
     return p;
 }
@@ -534,6 +652,7 @@ static int scan_sizes(const char* who, int dtype, int n, int length, int width) 
     return 0;
 }
 
+// floats: the partial rows of sum q, then the chunks' compositions
 extern "C" int64_t lego_gated_scan_workspace(int n, int length, int width) {
     if (n <= 0 || length <= 0 || width <= 0) return 0;
     const ScanPlan p = scan_plan(n, length, width);
@@ -554,15 +673,21 @@ extern "C" int lego_gated_scan_fwd(const void* x, int64_t x_sn, int64_t x_sl, co
                  "lego_gated_scan_fwd: workspace of %lld floats, lego_gated_scan_workspace says %lld", (long long)workspace_floats,
                  (long long)lego_gated_scan_workspace(n, length, width));
     const Seq sx{x, x_sn, x_sl}, sr{r, r_sn, r_sl}, si{i, i_sn, i_sl};
-    const bool full = width % SC_VC == 0;
     const dim3 grid(p.slices, n, p.chunks);
-#define GO(F, MODE) hipLaunchKernelGGL((scan_fwd_kernel<T, F, MODE>), grid, dim3(SC_THREADS), 0, ST, sx, sr, si, lam, sharpness, mask, mask_sn, state, \
-                                       (T*)h, last, tiles, workspace, length, width, p.chunks, p.per)
+#define GO(W, PASS) hipLaunchKernelGGL((scan_fwd_kernel<T, W, PASS>), grid, dim3(Fwd::THREADS), 0, ST, sx, sr, si, lam, sharpness, mask, mask_sn, state, \
+                                       (T*)h, last, tiles, workspace, length, width, p.per)
+#define BY_WIDTH(PASS)                          \
+    do {                                        \
+        if (width % 2 == 0) GO(EVEN, PASS);     \
+        else if (width > 1) GO(ODD, PASS);      \
+        else GO(SINGLE, PASS);                  \
+    } while (0)
     LEGO_BY_TYPE(dtype, {
-        if (p.chunks > 1) { if (full) GO(true, SUMMARY); else GO(false, SUMMARY); }
-        if (p.tiles > 1) { if (full) GO(true, TILES); else GO(false, TILES); }
-        else if (full) GO(true, ONE_TILE); else GO(false, ONE_TILE);
+        if (p.chunks > 1) BY_WIDTH(Pass::SUM);
+        if (p.tiles > 1) BY_WIDTH(Pass::TILES);
+        else BY_WIDTH(Pass::ONE);
     });
+#undef BY_WIDTH
 #undef GO
     return check_launch("lego_gated_scan_fwd");
 }
@@ -581,20 +706,27 @@ extern "C" int lego_gated_scan_bwd(const void* x, int64_t x_sn, int64_t x_sl, co
                  "lego_gated_scan_bwd: workspace of %lld floats, lego_gated_scan_workspace says %lld", (long long)workspace_floats,
                  (long long)lego_gated_scan_workspace(n, length, width));
     const Seq sx{x, x_sn, x_sl}, sr{r, r_sn, r_sl}, si{i, i_sn, i_sl}, sg{gh, gh_sn, gh_sl};
-    const bool full = width % SC_VC == 0;
-    float* qsum = workspace;
-    float* sums = workspace + (int64_t)p.rows * p.chunks * width;
+    float *qsum = workspace, *sums = workspace + (int64_t)p.rows * p.chunks * width;
     const dim3 all(p.slices, n, p.chunks), grid(p.slices, p.rows, p.chunks);
-#define GO(F, MODE, GRID) hipLaunchKernelGGL((scan_bwd_kernel<T, F, MODE>), GRID, dim3(SC_THREADS), 0, ST, sx, sr, si, sg, lam, sharpness, mask, mask_sn, \
-                                             tiles, glast, (T*)dx, (T*)dr, (T*)di, dstate, qsum, sums, n, length, width, p.chunks, p.per)
+#define SUM(W) hipLaunchKernelGGL((scan_bwd_sum_kernel<T, W>), all, dim3(Bwd::THREADS), 0, ST, sr, sg, lam, sharpness, mask, mask_sn, sums, length, width, p.per)
+#define GO(W) hipLaunchKernelGGL((scan_bwd_kernel<T, W>), grid, dim3(Bwd::THREADS), 0, ST, sx, sr, si, sg, lam, sharpness, mask, mask_sn, tiles, glast, d, \
+                                 dstate, qsum, sums, n, length, width, p.per)
+#define BY_WIDTH(LAUNCH)                   \
+    do {                                   \
+        if (width % 2 == 0) LAUNCH(EVEN);  \
+        else if (width > 1) LAUNCH(ODD);   \
+        else LAUNCH(SINGLE);               \
+    } while (0)
     LEGO_BY_TYPE(dtype, {
-        if (p.chunks > 1) { if (full) GO(true, SUMMARY, all); else GO(false, SUMMARY, all); }
-        if (p.tiles > 1) { if (full) GO(true, TILES, grid); else GO(false, TILES, grid); }
-        else if (full) GO(true, ONE_TILE, grid); else GO(false, ONE_TILE, grid);
+        const Grads<T> d = grads<T>(dx, dr, di);
+        if (p.chunks > 1) BY_WIDTH(SUM);
+        BY_WIDTH(GO);
     });
+#undef BY_WIDTH
 #undef GO
+#undef SUM
     if (int rc = check_launch("lego_gated_scan_bwd")) return rc;
-    hipLaunchKernelGGL(scan_dlam_kernel, dim3((width + 15) / 16), dim3(256), 0, ST, qsum, p.rows * p.chunks, lam, dlam, width);
+    hipLaunchKernelGGL(scan_dlam_kernel, dim3((width + 15) / 16), dim3(1024), 0, ST, qsum, p.rows * p.chunks, lam, dlam, width);
     return check_launch("lego_gated_scan_bwd (dlam)");
 }
 
