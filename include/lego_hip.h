@@ -422,7 +422,7 @@ int lego_gelu_bwd(const float* dg, const float* z, float* dz, int64_t n, void* s
  * A masked step keeps the state and its row of h is zeros.  h is contiguous; last [n, width] = the state behind the last step.
  * tiles [n, ceil(length / LEGO_SCAN_TILE), width]: the states that the backward pass starts from; NULL = not wanted.
  * _bwd: dx, dr, di (contiguous, zeros at masked steps), dlam [width], dstate [n, width] (NULL = not wanted) from gh = d h and glast = d last
- * (NULL = zeros).  length must be positive, n <= 65535.
+ * (NULL = zeros).  length must be positive, n <= 65535, strides between steps below 2^24 elements.
  * _step: one step of n states (mask NULL or [n]): h [n, width] in the activations' type and the new states `next` (may not alias `state`). */
 #define LEGO_SCAN_TILE 64
 int64_t lego_gated_scan_workspace(int n, int length, int width);                 /* floats, for _fwd and for _bwd */

@@ -311,6 +311,14 @@ def _last_dense(t: Optional[torch.Tensor]):
     return t if t is None or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
+def _steps(t: torch.Tensor):
+    """a sequence with dense channels whose steps the scan's 32-bit tile offsets reach, and its strides"""
+    t = _last_dense(t)
+    if t.shape[1] > 1 and t.stride(1) >= 1 << 24:
+        t = t.contiguous()
+    return t, (_at(t), t.stride(0), t.stride(1) if t.shape[1] > 1 else 0)
+
+
 def _bytes(mask: Optional[torch.Tensor]):
     """a mask of any type as bytes, 0 = not there (bool and uint8 as they are)"""
     if mask is None:
@@ -333,13 +341,12 @@ def gated_scan_fwd(x, r, i, lam, mask=None, state=None, sharpness=8.0, keep=Fals
     if length == 0:
         return h, torch.zeros(n, width, dtype=torch.float32, device=dev) if state is None else state.clone(memory_format=torch.contiguous_format), tiles
     last = torch.empty(n, width, dtype=torch.float32, device=dev)
-    x, r, i, mask = _last_dense(x), _last_dense(r), _last_dense(i), _bytes(mask)
+    (x, sx), (r, sr), (i, si), mask = _steps(x), _steps(r), _steps(i), _bytes(mask)
     lam, state = lam.contiguous(), None if state is None else state.contiguous()
     size = _lib.lib().lego_gated_scan_workspace(n, length, width)
     ws = _floats(size, dev)
-    _launch(x, "lego_gated_scan_fwd", _at(x), x.stride(0), x.stride(1), _at(r), r.stride(0), r.stride(1), _at(i), i.stride(0), i.stride(1),
-         _DTYPES[x.dtype], _at(lam), sharpness, _at(mask), 0 if mask is None else mask.stride(0), _at(state), _at(h), _at(last),
-         _at(tiles) if keep else None, _at(ws), size, n, length, width)
+    _launch(x, "lego_gated_scan_fwd", *sx, *sr, *si, _DTYPES[x.dtype], _at(lam), sharpness, _at(mask), 0 if mask is None else mask.stride(0),
+         _at(state), _at(h), _at(last), _at(tiles) if keep else None, _at(ws), size, n, length, width)
     return h, last, tiles
 
 
@@ -351,12 +358,11 @@ def gated_scan_bwd(gh, glast, x, r, i, lam, mask, tiles, sharpness=8.0):
         return dx, dr, di, torch.zeros(width, dtype=torch.float32, device=x.device), torch.zeros(n, width, dtype=torch.float32, device=x.device) \
             if glast is None else glast.clone(memory_format=torch.contiguous_format)
     dlam, dstate = torch.empty(width, dtype=torch.float32, device=x.device), torch.empty(n, width, dtype=torch.float32, device=x.device)
-    x, r, i, gh, mask = _last_dense(x), _last_dense(r), _last_dense(i), _last_dense(gh), _bytes(mask)
+    (x, sx), (r, sr), (i, si), (gh, sg), mask = _steps(x), _steps(r), _steps(i), _steps(gh), _bytes(mask)
     lam, glast = lam.contiguous(), None if glast is None else glast.contiguous()
     size = _lib.lib().lego_gated_scan_workspace(n, length, width)
     ws = _floats(size, x.device)
-    _launch(x, "lego_gated_scan_bwd", _at(x), x.stride(0), x.stride(1), _at(r), r.stride(0), r.stride(1), _at(i), i.stride(0), i.stride(1),
-         _at(gh), gh.stride(0), gh.stride(1), _DTYPES[x.dtype], _at(lam), sharpness, _at(mask), 0 if mask is None else mask.stride(0),
+    _launch(x, "lego_gated_scan_bwd", *sx, *sr, *si, *sg, _DTYPES[x.dtype], _at(lam), sharpness, _at(mask), 0 if mask is None else mask.stride(0),
          _at(tiles), _at(glast), _at(dx), _at(dr), _at(di), _at(dlam), _at(dstate), _at(ws), size, n, length, width)
     return dx, dr, di, dlam, dstate
 

@@ -165,6 +165,9 @@ def test_refusals_at_the_c_entry():
     assert fwd(0, 0, 5, 4) == 0 and fwd(0, 3, 5, 0) == 0                                      # nothing to do
     assert h.lego_gated_scan_bwd(one, z64, z64, one, z64, z64, one, z64, z64, one, z64, z64, 0, one, ctypes.c_float(8.0), None, z64, one, None, one, one,
                                  one, one, None, None, z64, 1, 5, 4, None) != 0 and "workspace" in err()
+    far = ctypes.c_int64(1 << 24)
+    assert h.lego_gated_scan_fwd(one, z64, far, one, z64, z64, one, z64, z64, 0, one, ctypes.c_float(8.0), None, z64, None, one, one, None, one,
+                                 ctypes.c_int64(1 << 20), 1, 5, 4, None) != 0 and "strides" in err()
     assert h.lego_gated_scan_step(one, z64, one, z64, one, z64, 0, one, ctypes.c_float(8.0), None, None, one, one, 1, 4, None) != 0 and "NULL" in err()
     norm = lambda o, wn, act, rows, width: h.lego_block_norm_fwd(one, z64, o, z64, None, z64, 0, act, one, one, wn, ctypes.c_float(1e-6), one, one,      # noqa: E731
                                                                  None, rows, width, None)
@@ -671,6 +674,19 @@ def _stack(seed=1, n=3, length=140, width=32, items=5000):
     return (_rand(seed, n, length, width).cuda(), _lam(width).cuda(), _rand(seed + 1, n, width).cuda(), _mask("prefix", n, length).cuda(),
             (1 + _rand(seed + 2, width, scale=0.1)).cuda(), _rand(seed + 3, width).cuda(), _rand(seed + 4, items, width).cuda(),
             torch.tensor([5, -1, 4999], device="cuda"))
+
+
+@pytest.mark.gpu
+def test_scan_steps_that_lie_far_apart():
+    """steps 2^24 elements apart, further than a tile's 32-bit offsets reach (one tensor of three is), and a single step with such a stride"""
+    far = torch.zeros((1 << 24) * 2 + 8, dtype=torch.float16, device="cuda").as_strided((1, 3, 8), (0, 1 << 24, 1))
+    x, r, i = (_rand(50 + q, 1, 3, 8, dtype=torch.float16).cuda() for q in range(3))
+    lam = _rand(53, 8).cuda()
+    far.copy_(x)
+    for length in (3, 1):
+        want, last = F.gated_scan(x[:, :length], r[:, :length], i[:, :length], lam)
+        got, state = F.gated_scan(far[:, :length], r[:, :length], i[:, :length], lam)
+        assert torch.equal(got, want) and torch.equal(state, last)
 
 
 @pytest.mark.gpu
