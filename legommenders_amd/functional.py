@@ -10,6 +10,7 @@ ROCm implementations only, and CPU tensors raise `LegoHipError` here before they
 from __future__ import annotations
 
 import itertools
+import math
 
 import torch
 
@@ -102,22 +103,22 @@ def _refuse(what, why):
 
 
 def _activations(what, first, *others):
-    """same shape, type and device for every activation"""
+    """same shape and type for every activation (the device of every operand is looked at where the pointers are taken)"""
     if not isinstance(first, torch.Tensor) or first.dtype not in _TYPES:
         _refuse(what, "activations are float32, bfloat16 or float16 tensors")
     for t in others:
-        if not isinstance(t, torch.Tensor) or t.shape != first.shape or t.dtype != first.dtype or t.device != first.device:
-            _refuse(what, f"every activation has to match the first: {tuple(first.shape)}, {first.dtype}, {first.device}")
+        if not isinstance(t, torch.Tensor) or t.shape != first.shape or t.dtype is not first.dtype:
+            _refuse(what, f"every activation has to match the first: {tuple(first.shape)}, {first.dtype}")
 
 
 def _weights(what, like, shape, *weights):
     for t in weights:
-        if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != torch.float32 or t.device != like.device:
+        if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not torch.float32:
             _refuse(what, f"weights and states are float32 tensors on {like.device}, here of shape {tuple(shape)}")
 
 
 def _mask_of(what, mask, shape, like):
-    if not isinstance(mask, torch.Tensor) or mask.shape != shape or mask.device != like.device:
+    if not isinstance(mask, torch.Tensor) or mask.shape != shape:
         _refuse(what, f"mask has to be of shape {tuple(shape)} on {like.device}")
 
 
@@ -149,8 +150,8 @@ def gated_scan(x, r, i, lam, mask=None, state=None, sharpness=8.0):
         _weights(what, x, (n, width), state)
     if mask is not None:
         _mask_of(what, mask, (n, length), x)
-    if not sharpness > 0:
-        _refuse(what, f"sharpness {sharpness} is not positive")
+    if not 0 < sharpness < math.inf:
+        _refuse(what, f"sharpness {sharpness} is not a positive number")
     _need_gpu(x, what)
     h, last, _ = _run(_ops.GatedScan, _ops.scan_op, (x, r, i, lam, state), x, r, i, lam, mask, state, float(sharpness), False)
     return h, last
@@ -167,8 +168,8 @@ def gated_scan_step(x, r, i, lam, state, mask=None, sharpness=8.0):
     _weights(what, x, x.shape, state)
     if mask is not None:
         _mask_of(what, mask, x.shape[:1], x)
-    if not sharpness > 0:
-        _refuse(what, f"sharpness {sharpness} is not positive")
+    if not 0 < sharpness < math.inf:
+        _refuse(what, f"sharpness {sharpness} is not a positive number")
     if torch.is_grad_enabled() and (x.requires_grad or r.requires_grad or i.requires_grad or lam.requires_grad or state.requires_grad):
         _refuse(what, "has no gradient; use gated_scan, or call it under torch.no_grad()")
     _need_gpu(x, what)
@@ -240,10 +241,9 @@ def token_logprobs(logits, targets=None, k=0, mask=None):
     if not isinstance(k, int) or not 0 <= k <= min(_ops.K.LOGPROBS_MAX_K, items):
         _refuse(what, f"k = {k} is not 0 to {min(_ops.K.LOGPROBS_MAX_K, items)}")
     if targets is not None and (not isinstance(targets, torch.Tensor) or targets.dtype not in (torch.int32, torch.int64)
-                                or targets.shape != logits.shape[:-1] or targets.device != logits.device):
+                                or targets.shape != logits.shape[:-1]):
         _refuse(what, f"targets are int32 or int64 of shape {tuple(logits.shape[:-1])} on {logits.device}")
-    if mask is not None and (not isinstance(mask, torch.Tensor) or mask.device != logits.device
-                             or (mask.shape != logits.shape and mask.shape != (items,))):
+    if mask is not None and (not isinstance(mask, torch.Tensor) or (mask.shape != logits.shape and mask.shape != (items,))):
         _refuse(what, f"mask has to be of shape {tuple(logits.shape)} or ({items},) on {logits.device}")
     _need_gpu(logits, what)
     flat = logits.dim() == 2

@@ -294,6 +294,31 @@ LOGPROBS_MAX_K = 128        # LEGO_LOGPROBS_MAX_K
 BLOCK_NORM_MAX_WIDTH = 16384
 
 
+def _bad(what, why):
+    raise _lib.LegoHipError(f"{what}: {why}")
+
+
+def _agree(what, x, like=(), floats=(), mask=None):
+    """what the pointers handed on rely on, for callers of the registered ops too: `like` as x in shape, type and device, `floats` (tensor, shape) fp32, a mask
+    of its shape, all on one GPU, sizes of 31 bits"""
+    device, dtype, shape = x.get_device(), x.dtype, x.shape
+    if dtype not in _DTYPES:
+        _bad(what, f"activations are float32, bfloat16 or float16, not {dtype}")
+    for size in shape:
+        if size >= 1 << 31:
+            _bad(what, f"sizes are below 2^31: {tuple(shape)}")
+    for t in like:
+        if t is not None and (t.dtype is not dtype or t.shape != shape or t.get_device() != device):
+            _bad(what, f"{tuple(t.shape)} {t.dtype} beside {tuple(shape)} {dtype} of one device")
+    for t, wanted in floats:
+        if t is not None and (t.dtype is not torch.float32 or t.shape != wanted or t.get_device() != device):
+            _bad(what, f"{tuple(t.shape)} {t.dtype} where {tuple(wanted)} float32 on {x.device} belongs")
+    if mask is not None and (mask[0].shape != mask[1] or mask[0].get_device() != device):
+        _bad(what, f"a mask of {tuple(mask[0].shape)} where {tuple(mask[1])} on {x.device} belongs")
+    if device < 0:
+        _bad(what, "tensors of a GPU: the HIP path has no CPU fallback")
+
+
 def _launch(t: torch.Tensor, name: str, *args):
     """the C entry on the device of `t`, and on that device's current stream"""
     device = t.device.index
@@ -335,6 +360,7 @@ def _floats(n, device, dtype=torch.float32):
 def gated_scan_fwd(x, r, i, lam, mask=None, state=None, sharpness=8.0, keep=False):
     """-> h [n, length, width], last [n, width] fp32, tiles (the backward pass's states; empty unless `keep`)"""
     n, length, width = x.shape
+    _agree("gated_scan", x, (r, i), ((lam, (width,)), (state, (n, width))), None if mask is None else (mask, (n, length)))
     dev = x.device
     h = torch.empty(n, length, width, dtype=x.dtype, device=dev)
     tiles = torch.empty(n, -(-length // SCAN_TILE) if keep else 0, width, dtype=torch.float32, device=dev)
@@ -353,6 +379,9 @@ def gated_scan_fwd(x, r, i, lam, mask=None, state=None, sharpness=8.0, keep=Fals
 def gated_scan_bwd(gh, glast, x, r, i, lam, mask, tiles, sharpness=8.0):
     """-> dx, dr, di (the activations' type), dlam, dstate (fp32)"""
     n, length, width = x.shape
+    _agree("gated_scan_bwd", x, (r, i, gh), ((lam, (width,)), (glast, (n, width)), (tiles, (n, -(-length // SCAN_TILE), width))),
+           None if mask is None else (mask, (n, length)))
+    tiles = tiles.contiguous()
     dx, dr, di = (torch.empty(n, length, width, dtype=x.dtype, device=x.device) for _ in range(3))
     if n == 0 or length == 0 or width == 0:
         return dx, dr, di, torch.zeros(width, dtype=torch.float32, device=x.device), torch.zeros(n, width, dtype=torch.float32, device=x.device) \
@@ -370,6 +399,7 @@ def gated_scan_bwd(gh, glast, x, r, i, lam, mask, tiles, sharpness=8.0):
 def gated_scan_step(x, r, i, lam, state, mask=None, sharpness=8.0):
     """-> h [n, width] in the activations' type, the new state [n, width] fp32"""
     n, width = x.shape
+    _agree("gated_scan_step", x, (r, i), ((lam, (width,)), (state, (n, width))), None if mask is None else (mask, (n,)))
     h, new = torch.empty(n, width, dtype=x.dtype, device=x.device), torch.empty(n, width, dtype=torch.float32, device=x.device)
     x, r, i, mask = _last_dense(x), _last_dense(r), _last_dense(i), _bytes(mask)
     lam, state = lam.contiguous(), state.contiguous()
@@ -389,6 +419,7 @@ def _ld(t):
 def block_norm_fwd(x, o, gate, post_w, scale, next_w, eps, act, keep=False):
     """2-D rows -> y, next (None where the half is absent), stat [halves, rows] (no columns unless `keep`)"""
     rows, width = x.shape
+    _agree("block_norm", x, (o, gate), ((post_w, (width,)), (scale, (width,)), (next_w, (width,))))
     dev = x.device
     y = torch.empty(rows, width, dtype=x.dtype, device=dev) if o is not None else None
     nxt = torch.empty(rows, width, dtype=x.dtype, device=dev) if next_w is not None else None
@@ -403,6 +434,9 @@ def block_norm_fwd(x, o, gate, post_w, scale, next_w, eps, act, keep=False):
 def block_norm_bwd(dy, dn, x, o, gate, post_w, scale, next_w, eps, act, stat):
     """-> dx, do, dgate (the activations' type), dpost_w, dscale, dnext_w (fp32); None where the operand is absent"""
     rows, width = x.shape
+    _agree("block_norm_bwd", x, (o, gate, dy, dn), ((post_w, (width,)), (scale, (width,)), (next_w, (width,)),
+                                                    (stat, ((o is not None) + (next_w is not None), rows))))
+    stat = stat.contiguous()
     new = lambda t: None if t is None else torch.empty(rows, width, dtype=x.dtype, device=x.device)      # noqa: E731
     dx, do, dgate = new(x), new(o), new(gate)
     make = torch.zeros if rows == 0 else torch.empty
@@ -419,9 +453,16 @@ def block_norm_bwd(dy, dn, x, o, gate, post_w, scale, next_w, eps, act, stat):
     return dx, do, dgate, dpw, dsc, dnw
 
 
+def _check_targets(what, targets, rows, logits):
+    if targets is not None and (targets.dtype not in (torch.int32, torch.int64) or targets.shape != (rows,) or targets.get_device() != logits.get_device()):
+        _bad(what, f"targets are int32 or int64 of [{rows}] on {logits.device}, not {tuple(targets.shape)} {targets.dtype}")
+
+
 def token_logprobs_fwd(logits, targets, k=0, mask=None):
     """2-D logits -> logp, entropy [rows], stat [rows, 2] (maximum, ln of the sum), top [rows, k] fp32, index [rows, k] int32"""
     rows, items = logits.shape
+    _agree("token_logprobs", logits, mask=None if mask is None else (mask, (rows, items)))
+    _check_targets("token_logprobs", targets, rows, logits)
     f = dict(dtype=torch.float32, device=logits.device)
     logp, entropy, stat = torch.empty(rows, **f), torch.empty(rows, **f), torch.empty(rows, 2, **f)
     top, index = torch.empty(rows, k, **f), torch.empty(rows, k, dtype=torch.int32, device=logits.device)
@@ -438,12 +479,19 @@ def token_logprobs_fwd(logits, targets, k=0, mask=None):
 def token_logprobs_bwd(g_logp, g_entropy, g_top, logits, targets, mask, stat, entropy, index):
     """-> d logits [rows, items], in their type; a gradient that is None counts as zeros"""
     rows, items = logits.shape
+    k = index.shape[-1]
+    if g_top is not None and g_top.numel() == 0:
+        g_top = None
+    _agree("token_logprobs_bwd", logits, (), ((g_logp, (rows,)), (g_entropy, (rows,)), (g_top, (rows, k)), (stat, (rows, 2)), (entropy, (rows,))),
+           None if mask is None else (mask, (rows, items)))
+    _check_targets("token_logprobs_bwd", targets, rows, logits)
+    if index.dtype is not torch.int32 or index.shape != (rows, k) or index.get_device() != logits.get_device():
+        _bad("token_logprobs_bwd", f"index is int32 [{rows}, k], not {tuple(index.shape)} {index.dtype}")
+    stat, entropy, index = stat.contiguous(), entropy.contiguous(), index.contiguous()
     out = torch.empty(rows, items, dtype=logits.dtype, device=logits.device)
     logits, mask = _last_dense(logits), _bytes(mask)
     targets, g_logp, g_entropy, g_top = (None if t is None else t.contiguous() for t in (targets, g_logp, g_entropy, g_top))
-    if g_top is not None and g_top.numel() == 0:
-        g_top = None
     _launch(logits, "lego_token_logprobs_bwd", _at(logits), logits.stride(0), _DTYPES[logits.dtype], _at(mask), 0 if mask is None else mask.stride(0),
-         _at(targets), int(targets is not None and targets.dtype == torch.int64), index.shape[1], _at(stat), _at(entropy), _at(index),
+         _at(targets), int(targets is not None and targets.dtype == torch.int64), k, _at(stat), _at(entropy), _at(index),
          _at(g_logp), _at(g_entropy), _at(g_top), _at(out), rows, items)
     return out

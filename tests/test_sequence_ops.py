@@ -185,6 +185,32 @@ def test_refusals_at_the_c_entry():
     assert lp(0, 8, rows=0) == 0
 
 
+def test_refusals_below_the_public_functions():
+    """the registered ops end here: what the pointers rely on is looked at for them too, before anything is launched"""
+    x, w, bad = torch.zeros(2, 70, 8), torch.zeros(8), torch.zeros(8, dtype=torch.float64)
+    st, tiles = torch.zeros(2, 8), torch.zeros(2, 2, 8)
+    for call in [lambda: K.gated_scan_fwd(x, x, x, bad), lambda: K.gated_scan_fwd(x, x[:1], x, w), lambda: K.gated_scan_fwd(x, x, x.half(), w),
+                 lambda: K.gated_scan_fwd(x, x, x, w, torch.ones(2, 69)), lambda: K.gated_scan_fwd(x, x, x, w, None, st[:1]),
+                 lambda: K.gated_scan_bwd(x, None, x, x, x, w, None, tiles[:, :1]), lambda: K.gated_scan_bwd(x[:, :1], None, x, x, x, w, None, tiles),
+                 lambda: K.gated_scan_step(st, st, st, w[:4], st), lambda: K.gated_scan_step(st, st, st, w, st.half()),
+                 lambda: K.gated_scan_step(st, st, st, w, st, torch.ones(3)), lambda: K.gated_scan_fwd(x, x, x, w)]:
+        with pytest.raises(LegoHipError, match="gated_scan"):
+            call()
+    stat = torch.zeros(2, 2)
+    for call in [lambda: K.block_norm_fwd(st, st, None, w, w, bad, 1e-6, 0), lambda: K.block_norm_fwd(st, st[:1], None, w, w, w, 1e-6, 0),
+                 lambda: K.block_norm_bwd(st, st, st, st, None, w, w, w, 1e-6, 0, stat[:1]), lambda: K.block_norm_fwd(st, st, st, w, w, w, 1e-6, 2),
+                 lambda: K.block_norm_fwd(torch.empty(1 << 31, 1, device="meta"), None, None, None, None, w[:1], 1e-6, 0)]:
+        with pytest.raises(LegoHipError, match="block_norm"):
+            call()
+    t, index = torch.zeros(2, dtype=torch.int64), torch.zeros(2, 3, dtype=torch.int32)
+    for call in [lambda: K.token_logprobs_fwd(st, t[:1]), lambda: K.token_logprobs_fwd(st, t.float()), lambda: K.token_logprobs_fwd(st, t, 3, st[:1]),
+                 lambda: K.token_logprobs_fwd(st.double(), t), lambda: K.token_logprobs_fwd(torch.empty(1 << 31, 1, device="meta"), None),
+                 lambda: K.token_logprobs_bwd(None, None, torch.zeros(2, 2), st, t, None, stat, w[:2], index),
+                 lambda: K.token_logprobs_bwd(w[:2], None, None, st, t, None, stat, w[:2], index.long()), lambda: K.token_logprobs_fwd(st, t, 3)]:
+        with pytest.raises(LegoHipError, match="token_logprobs"):
+            call()
+
+
 def test_workspaces_cover_what_the_kernels_index():
     h = _lib.lib()
     for n, length, width in [(1, 1, 1), (1, 10007, 301), (2, 32768, 768), (64, 50, 256), (65535, 3, 4), (1, 64 * 5 + 1, 1 << 12)]:
@@ -687,6 +713,19 @@ def test_scan_steps_that_lie_far_apart():
         want, last = F.gated_scan(x[:, :length], r[:, :length], i[:, :length], lam)
         got, state = F.gated_scan(far[:, :length], r[:, :length], i[:, :length], lam)
         assert torch.equal(got, want) and torch.equal(state, last)
+
+
+@pytest.mark.gpu
+def test_operands_of_another_device_are_refused():
+    x, w, t = _rand(1, 2, 3, 8).cuda(), _rand(2, 8).cuda(), torch.zeros(2, 3, dtype=torch.int64)
+    for grad in (False, True):
+        x = x.detach().requires_grad_(grad)
+        for call in [lambda: F.gated_scan(x, x, x, w.cpu()), lambda: F.gated_scan(x, x.detach().cpu(), x, w), lambda: F.rms_norm(x, w.cpu()),
+                     lambda: F.gated_scan(x, x, x, w, mask=torch.ones(2, 3)), lambda: F.gated_residual_norm(x, x, x, w, w.cpu(), w),
+                     lambda: F.token_logprobs(x, t), lambda: F.token_logprobs(x, mask=torch.ones(8)),
+                     lambda: F.gated_scan_step(x.detach()[0], x.detach()[0], x.detach()[0], w, torch.zeros(3, 8))]:
+            with pytest.raises(LegoHipError):
+                call()
 
 
 @pytest.mark.gpu
