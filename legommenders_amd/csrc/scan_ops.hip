@@ -11,8 +11,8 @@
 // formed again from it in fp32, and G_t = dh_t + a_(t+1) G_(t+1) is the same composition from the other end.
 //
 // What bounds it: memory from about 192 workgroups on (64 x 2048 x 256 fp32: forward 109 us, 4.9 TB/s; backward 217 us, 4.3 TB/s); in bf16, with half the
-// bytes, the exponentials and the waits of 16 waves a CU (forward 187 us for 2 x 32768 x 768, its inputs read twice: 3.8 TB/s).  512 x 50 x 256 fp32 with
-// ragged lengths: 19 us forward, 40 backward.
+// bytes, vector instructions (70 % of the time; 40 a cell, 5 of them transcendental) (forward 79 us of 54 for the same cells, 170 us for 2 x 32768 x 768, its inputs read twice: 4.1 TB/s).  512 x 50 x 256 fp32 with
+// ragged lengths: 18 us forward, 41 backward.
 #include <type_traits>
 
 #include "seq_common.hpp"
@@ -116,36 +116,43 @@ template <typename S> struct Lane {
 
 template <typename S> struct Totals { fv a[2][S::WAVES][SC_LANES], h[2][S::WAVES][SC_LANES]; };      // two tiles in turn: one barrier a tile is enough
 
-// The compositions of a tile's runs, in the order DIR (1: from the first run, -1: from the last).  put: this lane's (A, H), a barrier, get: the
-// composition (pa, ph) of the runs before this lane's and (ta, th) of the whole tile.
+// A tile's runs, in the order DIR (1: from the first run, -1: from the last).  put: this lane's (A, H), a barrier; then before: the state that enters this
+// lane's run, if `carry` enters the tile -- it moves on to what leaves it -- or past, for a chunk's composition (through, carry).  The waves pass on a
+// state, two multiply-adds each; composing them as the lanes are composed took 64 instructions more a tile, of 400 (64 x 2048 x 256 bf16 forward 87
+// -> 79 us, 2 x 32768 x 768 177 -> 170).
 template <typename S, int DIR>
 struct Join {
-    fv pa, ph, ta, th;
-    static __device__ __forceinline__ fv before(fv v, int groups) { return DIR > 0 ? shuffle_up(v, SC_LANES * groups) : shuffle_down(v, SC_LANES * groups); }
+    fv pa, ph;                                                         // the composition of the wave's runs before this lane's
+    static __device__ __forceinline__ fv shifted(fv v, int groups) { return DIR > 0 ? shuffle_up(v, SC_LANES * groups) : shuffle_down(v, SC_LANES * groups); }
     __device__ __forceinline__ void put(Totals<S>& tot, int buf, const Lane<S>& at, fv A, fv H) {
         const int place = DIR > 0 ? at.group : SC_GROUPS - 1 - at.group;
 #pragma unroll
         for (int by = 1; by < SC_GROUPS; by <<= 1) {
-            const fv a = before(A, by), h = before(H, by);
+            const fv a = shifted(A, by), h = shifted(H, by);
             if (place >= by) { H = A * h + H; A = A * a; }
         }
         if (place == SC_GROUPS - 1) { tot.a[buf][at.wave][at.cl] = A; tot.h[buf][at.wave][at.cl] = H; }
-        pa = before(A, 1), ph = before(H, 1);
+        pa = shifted(A, 1), ph = shifted(H, 1);
         if (place == 0) { pa = fv(1.f); ph = fv(0.f); }
     }
-    __device__ __forceinline__ void get(const Totals<S>& tot, int buf, const Lane<S>& at) {
-        ta = fv(1.f), th = fv(0.f);
-        fv wa = ta, wh = th;
-#pragma unroll 4
+    __device__ __forceinline__ fv before(const Totals<S>& tot, int buf, const Lane<S>& at, fv& carry) const {
+        fv mine = carry;
+#pragma unroll
         for (int q = 0; q < S::WAVES; ++q) {
             const int w = DIR > 0 ? q : S::WAVES - 1 - q;
-            if (w == at.wave) { wa = ta; wh = th; }
-            const fv a = tot.a[buf][w][at.cl], h = tot.h[buf][w][at.cl];
-            th = a * th + h;
-            ta = a * ta;
+            if (w == at.wave) mine = carry;
+            carry = tot.a[buf][w][at.cl] * carry + tot.h[buf][w][at.cl];
         }
-        ph = pa * wh + ph;
-        pa = pa * wa;
+        return pa * mine + ph;
+    }
+    static __device__ __forceinline__ void past(const Totals<S>& tot, int buf, const Lane<S>& at, fv& through, fv& carry) {
+#pragma unroll
+        for (int q = 0; q < S::WAVES; ++q) {
+            const int w = DIR > 0 ? q : S::WAVES - 1 - q;
+            const fv a = tot.a[buf][w][at.cl];
+            carry = a * carry + tot.h[buf][w][at.cl];
+            through = a * through;
+        }
     }
 };
 
@@ -176,11 +183,13 @@ struct Rows {
 // flight, and a tile's wait leaves the next tile's loads alone); what is not live reads the tile's head row again, which costs no traffic.
 template <typename T, int N, int STEPS, Width W>
 struct Steps {
-    vec<T, SC_VC> v[N][STEPS];
+    using Pair = vec<T, SC_VC>;
+    using Bits = typename std::conditional<sizeof(Pair) == 4, uint32_t, uint64_t>::type;
+    Pair v[N][STEPS];
     uint32_t live;                                                     // bit s: step s exists and is not masked (looked at where !whole only)
-    bool whole;                                                        // every step of the tile is live
+    bool whole;                                                        // every step of the wave is live
     bool second;                                                       // (ODD) of what was loaded, only the second is a channel of this lane
-    static __device__ __forceinline__ void one(vec<T, SC_VC>& to, const char* p) { __builtin_memcpy(&to, p, (W == SINGLE ? 1 : SC_VC) * sizeof(T)); }
+    static __device__ __forceinline__ void one(Pair& to, const char* p) { __builtin_memcpy(&to, p, (W == SINGLE ? 1 : SC_VC) * sizeof(T)); }
     // t: this lane's first step in the tile, left: steps from the tile's head to the end (at least 1), mask: of the tile's head
     __device__ __forceinline__ void fetch(const Rows<T, N, W>& rows, const uint8_t* __restrict__ mask, int t, int left, int c, int width) {
         second = c + 1 == width;
@@ -210,25 +219,29 @@ struct Steps {
                 const uint32_t at = live >> s & 1u ? rows.at[q] + s * rows.step[q] : rows.idle[q];
                 one(v[q][s], reinterpret_cast<const char*>(rows.head[q]) + at);
             }
+        whole = __all(live == (1u << STEPS) - 1u);                     // (of this wave's steps: then nothing has to be cleaned)
     }
     __device__ __forceinline__ fv at(int q, int s) const { return __builtin_convertvector(v[q][s], fv); }
     // A step that is not live: the recurrence gate's logit R becomes -inf -- sigmoid 0, decay 1, beta 0 exactly -- and the other inputs 0, so that
     // nothing after this asks again whether a step is live, but for what is written
     template <int R>
+    // (64 x 2048 x 256 bf16 with a mask: 92 us with selects of single channels and every tile of a mask cleaned, 77 so)
     __device__ __forceinline__ void clean() {
         if constexpr (W == ODD)
 #pragma unroll
             for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-                for (int q = 0; q < N; ++q) v[q][s][0] = second ? v[q][s][1] : v[q][s][0];
+                for (int q = 0; q < N; ++q) {
+                    const Bits b = __builtin_bit_cast(Bits, v[q][s]);
+                    v[q][s] = __builtin_bit_cast(Pair, second ? b >> 8 * sizeof(T) : b);
+                }
         if (whole) return;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
             const bool on = live >> s & 1u;
 #pragma unroll
-            for (int q = 0; q < N; ++q)
-#pragma unroll
-                for (int k = 0; k < SC_VC; ++k) v[q][s][k] = on ? v[q][s][k] : (T)(q == R ? -INFINITY : 0.f);
+            for (int q = 0; q < N; ++q)                                // both channels at once
+                v[q][s] = __builtin_bit_cast(Pair, on ? __builtin_bit_cast(Bits, v[q][s]) : q == R ? __builtin_bit_cast(Bits, Pair((T)-INFINITY)) : (Bits)0);
         }
     }
     __device__ __forceinline__ fv kept(int s, fv f) const {            // what is written, or summed over steps
@@ -236,14 +249,13 @@ struct Steps {
     }
     // hides from the compiler that the values are still the same: what is cheap to form from them is formed again, not kept in registers
     __device__ __forceinline__ void renew() {
-        using Bits = typename std::conditional<SC_VC * sizeof(T) == 4, uint32_t, uint64_t>::type;
 #pragma unroll
         for (int q = 0; q < N; ++q)
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
                 Bits b = __builtin_bit_cast(Bits, v[q][s]);
                 asm volatile("" : "+v"(b));
-                v[q][s] = __builtin_bit_cast(decltype(v[q][s] + v[q][s]), b);
+                v[q][s] = __builtin_bit_cast(Pair, b);
             }
     }
 };
@@ -264,8 +276,8 @@ __device__ __forceinline__ fv entering(Totals<S>& tot, const float* __restrict__
     Join<S, 1> j;
     j.put(tot, 1, at, A, H);                                           // (the first tile uses the other half)
     __syncthreads();
-    j.get(tot, 1, at);
-    return j.ta * edge + j.th;
+    j.before(tot, 1, at, edge);
+    return edge;
 }
 
 // the byte offset of step t, channel c in a tile of a contiguous output
@@ -351,13 +363,11 @@ __global__ __launch_bounds__(Fwd::THREADS, 4) void scan_fwd_kernel(Seq x, Seq r,
         Join<S, 1> j;
         j.put(tot, buf, at, A, H);
         __syncthreads();
-        j.get(tot, buf, at);
-        if constexpr (PASS == Pass::SUM) through = j.ta * through;
+        if constexpr (PASS == Pass::SUM) j.past(tot, buf, at, through, carry);
         else {
             if (tiles != nullptr && at.run == 0) store<float, SC_VC, FULL>(tiles + (n * n_tiles + tile) * width, c, width, carry);
-            replay<T, FULL>(in.whole, in.live, some, a, b, j.pa * carry + j.ph, h + (n * length + (int64_t)tile * SC_TILE) * width, at_h, t, left, c, width);
+            replay<T, FULL>(in.whole, in.live, some, a, b, j.before(tot, buf, at, carry), h + (n * length + (int64_t)tile * SC_TILE) * width, at_h, t, left, c, width);
         }
-        carry = j.ta * carry + j.th;
         if (PASS == Pass::ONE || tile + 1 == end) break;
         in = ahead;
     }
@@ -492,9 +502,7 @@ __global__ __launch_bounds__(Bwd::THREADS, 2) void scan_bwd_sum_kernel(Seq r, Se
         Join<S, -1> j;
         j.put(tot, buf, at, A, C);
         __syncthreads();
-        j.get(tot, buf, at);
-        through = j.ta * through;
-        carry = j.ta * carry + j.th;
+        j.past(tot, buf, at, through, carry);
         if (tile == first) break;
         in = ahead;
     }
@@ -535,7 +543,7 @@ __global__ __launch_bounds__(Bwd::THREADS, 2) void scan_bwd_kernel(Seq x, Seq r,
         rows.set(2, x, n, tile, t, c, width);
         rows.set(3, i, n, tile, t, c, width);
         in.fetch(rows, mask != nullptr ? mask + n * mask_sn + (int64_t)tile * SC_TILE : nullptr, t, left, c, width);
-        const fv head = load<float, SC_VC, FULL>(tiles + (n * n_tiles + tile) * width, c, width);
+        fv head = load<float, SC_VC, FULL>(tiles + (n * n_tiles + tile) * width, c, width);
         fv sr[S::STEPS], si[S::STEPS], a[S::STEPS], beta[S::STEPS], A, H, C;
         const bool some = compose_both(in, near, k, sr, si, a, beta, A, H, C);
         Join<S, 1> f;
@@ -543,10 +551,7 @@ __global__ __launch_bounds__(Bwd::THREADS, 2) void scan_bwd_kernel(Seq x, Seq r,
         f.put(fwd, buf, at, A, H);
         j.put(tot, buf, at, A, C);
         __syncthreads();
-        f.get(fwd, buf, at);
-        j.get(tot, buf, at);
-        const fv now = f.pa * head + f.ph, back = j.pa * carry + j.ph;
-        carry = j.ta * carry + j.th;
+        const fv now = f.before(fwd, buf, at, head), back = j.before(tot, buf, at, carry);
         if (tile == 0 && at.run == 0 && dstate != nullptr) store<float, SC_VC, FULL>(dstate + n * width, c, width, carry);
         gradients<T, FULL>(in, some, k, sr, si, a, beta, now, back, q_all, d, (n * length + (int64_t)tile * SC_TILE) * width, at_d, t, left, c, width);
         if (--tile < first) {
