@@ -512,8 +512,11 @@ __global__ __launch_bounds__(Bwd::THREADS, 2) void scan_bwd_sum_kernel(Seq r, Se
     store<float, SC_VC, FULL>(s + width, c, width, carry);
 }
 
-// Workgroup: channels [64 blockIdx.x, + 64) of sequences blockIdx.y, + gridDim.y, .., tiles [per blockIdx.z, + per) from the last one on
-template <typename T, Width W>
+// Workgroup: channels [64 blockIdx.x, + 64) of sequences blockIdx.y, + gridDim.y, .., tiles [per blockIdx.z, + per) from the last one on.
+// AHEAD: the next tile's loads are in flight while a tile is computed.  Its registers are there for 16-bit inputs only, and it pays from 4 tiles a
+// workgroup on: bf16 without and with, 64 x 2048 x 256 166 / 150 us, 2 x 32768 x 768 250 / 228, 512 x 50 x 256 35.6 / 37.3; 1 x 10007 x 301 fp16, 2 tiles
+// a workgroup, 33.8 / 36.0.
+template <typename T, Width W, bool AHEAD>
 __global__ __launch_bounds__(Bwd::THREADS, 2) void scan_bwd_kernel(Seq x, Seq r, Seq i, Seq gh, const float* __restrict__ lam, float sharpness,
                                                                    const uint8_t* __restrict__ mask, int64_t mask_sn, const float* __restrict__ tiles,
                                                                    const float* __restrict__ glast, Grads<T> d, float* __restrict__ dstate,
@@ -530,19 +533,25 @@ __global__ __launch_bounds__(Bwd::THREADS, 2) void scan_bwd_kernel(Seq x, Seq r,
     const uint32_t at_d = lane_offset<T>(t, width, c);
     fv q_all(0.f), carry(0.f);
     Rows<T, 4, W> rows;
-    Steps<T, 4, S::STEPS, W> in;
+    Steps<T, 4, S::STEPS, W> in, ahead;
+    const auto fetch = [&](int64_t n, int tile, Steps<T, 4, S::STEPS, W>& to) {
+        rows.set(0, r, n, tile, t, c, width);
+        rows.set(1, gh, n, tile, t, c, width);
+        rows.set(2, x, n, tile, t, c, width);
+        rows.set(3, i, n, tile, t, c, width);
+        to.fetch(rows, mask != nullptr ? mask + n * mask_sn + (int64_t)tile * SC_TILE : nullptr, t, length - tile * SC_TILE, c, width);
+    };
     int tile = end - 1;
     int64_t n = blockIdx.y;
     if (glast != nullptr) carry = load<float, SC_VC, FULL>(glast + n * width, c, width);
     if (end < n_tiles) carry = entering<FULL, -1>(tot, sums + n * chunks * 2 * width, chunks - 1, chunks - 1 - (int)blockIdx.z, carry, at, width);
     // (sequences that are cut have a workgroup each, so that what follows takes no second one of them.)  One loop over sequences and tiles: nested, the compiler spills 45 registers
+    if constexpr (AHEAD) fetch(n, tile, in);
     for (int buf = 0; n < seqs; buf ^= 1) {
         const int left = length - tile * SC_TILE;
-        rows.set(0, r, n, tile, t, c, width);
-        rows.set(1, gh, n, tile, t, c, width);
-        rows.set(2, x, n, tile, t, c, width);
-        rows.set(3, i, n, tile, t, c, width);
-        in.fetch(rows, mask != nullptr ? mask + n * mask_sn + (int64_t)tile * SC_TILE : nullptr, t, left, c, width);
+        // (behind the last tile some tile again, rather than a branch: with one the compiler spills)
+        if constexpr (AHEAD) fetch(tile > first ? n : min(n + (int64_t)gridDim.y, (int64_t)seqs - 1), tile > first ? tile - 1 : end - 1, ahead);
+        else fetch(n, tile, in);
         fv head = load<float, SC_VC, FULL>(tiles + (n * n_tiles + tile) * width, c, width);
         fv sr[S::STEPS], si[S::STEPS], a[S::STEPS], beta[S::STEPS], A, H, C;
         const bool some = compose_both(in, near, k, sr, si, a, beta, A, H, C);
@@ -554,6 +563,7 @@ __global__ __launch_bounds__(Bwd::THREADS, 2) void scan_bwd_kernel(Seq x, Seq r,
         const fv now = f.before(fwd, buf, at, head), back = j.before(tot, buf, at, carry);
         if (tile == 0 && at.run == 0 && dstate != nullptr) store<float, SC_VC, FULL>(dstate + n * width, c, width, carry);
         gradients<T, FULL>(in, some, k, sr, si, a, beta, now, back, q_all, d, (n * length + (int64_t)tile * SC_TILE) * width, at_d, t, left, c, width);
+        if constexpr (AHEAD) in = ahead;
         if (--tile < first) {
             tile = end - 1;
             n += gridDim.y;
@@ -714,7 +724,7 @@ extern "C" int lego_gated_scan_bwd(const void* x, int64_t x_sn, int64_t x_sl, co
     float *qsum = workspace, *sums = workspace + (int64_t)p.rows * p.chunks * width;
     const dim3 all(p.slices, n, p.chunks), grid(p.slices, p.rows, p.chunks);
 #define SUM(W) hipLaunchKernelGGL((scan_bwd_sum_kernel<T, W>), all, dim3(Bwd::THREADS), 0, ST, sr, sg, lam, sharpness, mask, mask_sn, sums, length, width, p.per)
-#define GO(W) hipLaunchKernelGGL((scan_bwd_kernel<T, W>), grid, dim3(Bwd::THREADS), 0, ST, sx, sr, si, sg, lam, sharpness, mask, mask_sn, tiles, glast, d, \
+#define GO(W) hipLaunchKernelGGL((scan_bwd_kernel<T, W, ahead>), grid, dim3(Bwd::THREADS), 0, ST, sx, sr, si, sg, lam, sharpness, mask, mask_sn, tiles, glast, d, \
                                  dstate, qsum, sums, n, length, width, p.per)
 #define BY_WIDTH(LAUNCH)                   \
     do {                                   \
@@ -725,7 +735,12 @@ extern "C" int lego_gated_scan_bwd(const void* x, int64_t x_sn, int64_t x_sl, co
     LEGO_BY_TYPE(dtype, {
         const Grads<T> d = grads<T>(dx, dr, di);
         if (p.chunks > 1) BY_WIDTH(SUM);
-        BY_WIDTH(GO);
+        const auto run = [&](auto with) {
+            constexpr bool ahead = decltype(with)::value;
+            BY_WIDTH(GO);
+        };
+        if (sizeof(T) == 2 && p.per >= 4) run(std::integral_constant<bool, sizeof(T) == 2>());
+        else run(std::false_type());
     });
 #undef BY_WIDTH
 #undef GO

@@ -322,6 +322,15 @@ def test_scan_and_its_gradients(shape, mask, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape,mask,dtype",
+                         [((200, 260, 24), m, t) for m in (None, "prefix", "holes") for t in TYPES] +          # a workgroup a sequence, 5 tiles each
+                         [((190, 1280, 24), m, torch.bfloat16) for m in (None, "prefix")] +                    # chunks of 4 tiles
+                         [((52, 193, 2561), "prefix", torch.float16), ((52, 193, 2561), None, torch.float32)])    # backward: workgroups with two sequences
+def test_scan_of_many_sequences(shape, mask, dtype):
+    test_scan_and_its_gradients(shape, mask, dtype)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("mask_type", [torch.bool, torch.uint8, torch.int32, torch.int64, torch.float32])
 def test_scan_takes_masks_of_any_type_and_strided_everything(mask_type):
     n, length, width = 3, 70, 12
