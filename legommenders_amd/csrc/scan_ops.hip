@@ -10,9 +10,9 @@
 // The backward pass keeps no h: the forward pass saves the fp32 state at the head of every tile (1/64 of the cells), the tile's states are
 // formed again from it in fp32, and G_t = dh_t + a_(t+1) G_(t+1) is the same composition from the other end.
 //
-// What bounds it: memory from about 192 workgroups on (64 x 2048 x 256 fp32: forward 109 us, 4.9 TB/s; backward 217 us, 4.3 TB/s); in bf16, with half the
-// bytes, vector instructions (70 % of the time; 40 a cell, 5 of them transcendental) (forward 79 us of 54 for the same cells, 170 us for 2 x 32768 x 768, its inputs read twice: 4.1 TB/s).  512 x 50 x 256 fp32 with
-// ragged lengths: 18 us forward, 41 backward.
+// What bounds it: in fp32 memory (64 x 2048 x 256: forward 110 us, 4.9 TB/s; backward 204 us, 4.6 TB/s); in 16 bits, with half the bytes, the vector
+// units (forward 74 us of 54 for the same cells: 50 instructions a cell, 5 of them transcendental).  Cut into chunks, 2 x 32768 x 768 bf16: forward
+// 170 us, backward 228.  512 x 50 x 256 fp32 with ragged lengths: 18 us forward, 39 backward.
 #include <type_traits>
 
 #include "seq_common.hpp"
@@ -42,7 +42,7 @@ __device__ __forceinline__ float softplus(float v) {
     return v > 20.f ? v : s;
 }
 
-// l = k sigmoid(r) <= 0, a = e^l, beta = sqrt(1 - a^2) = sqrt((1 - a)(1 + a)), 4 channels.  1 - a would cancel near 1: for l >= -0.5
+// l = k sigmoid(r) <= 0, a = e^l, beta = sqrt(1 - a^2) = sqrt((1 - a)(1 + a)), 2 channels.  1 - a would cancel near 1: for l >= -0.5
 // (e^l - 1) / l is the degree-5 polynomial through its Chebyshev points there (3e-9 relative), else the hardware exponential.  NEAR: |k| <= 0.5
 // for every channel of the wave, so that no l is below -0.5 (decays that start at 0.6 and more -- the usual initialisation is 0.9 to 0.999).
 template <bool NEAR>
@@ -545,7 +545,8 @@ __global__ __launch_bounds__(Bwd::THREADS, 2) void scan_bwd_kernel(Seq x, Seq r,
     int64_t n = blockIdx.y;
     if (glast != nullptr) carry = load<float, SC_VC, FULL>(glast + n * width, c, width);
     if (end < n_tiles) carry = entering<FULL, -1>(tot, sums + n * chunks * 2 * width, chunks - 1, chunks - 1 - (int)blockIdx.z, carry, at, width);
-    // (sequences that are cut have a workgroup each, so that what follows takes no second one of them.)  One loop over sequences and tiles: nested, the compiler spills 45 registers
+    // (Sequences that are cut have a workgroup each: what follows takes no second one of them.)  One loop over sequences and tiles: nested, the compiler
+    // spills 45 registers.
     if constexpr (AHEAD) fetch(n, tile, in);
     for (int buf = 0; n < seqs; buf ^= 1) {
         const int left = length - tile * SC_TILE;
@@ -624,20 +625,26 @@ __global__ __launch_bounds__(256) void scan_step_kernel(Seq x, Seq r, Seq i, con
 
 struct ScanPlan { int slices, tiles, chunks, per, rows; };
 
-// One workgroup a (sequence, 64 channels) streams as fast as memory gives from about 192 of them on: 256 workgroups, 64 x 2048 x 256 fp32, 109 us forward
-// and 217 backward against 196 and 289 cut into chunks, which read their inputs twice.  Below that sequences of 4 tiles and more are cut until about
-// CUT_TO workgroups are in flight, a tile each at least.  Forward + backward (us) for 512 / 768 / 1024: 2 x 32768 x 768 bf16 430 / 432 / 442,
-// 8 x 4096 x 768 bf16 250 / 224 / 225; at least 1 / 2 / 4 tiles: 1 x 10007 x 301 fp16 62 / 70 / 78, 1 x 2048 x 256 fp32 26 / 34 / 51.  (A single pass
-// over the chunks, each waiting for the one before it, was no faster, 184 + 284 us for the first: what a tile waits for the words of others costs more
+// A workgroup a (sequence, 64 channels) reads every input once, and from some number of them on is as fast as memory or the vector units allow; fewer
+// leave the GPU idle, and sequences of 4 tiles and more are then cut into chunks, which read their inputs twice.  n x 2048 x 256, us uncut / cut:
+//   workgroups        64         128         160         192         224         256
+//   forward   fp32   72 / 49    78 / 95     84 / 120    90 / 146   100 / 177   112 / 194      cut below  96
+//   forward   bf16   63 / 37    64 / 63     66 / 76     66 / 84     66 / 103    68 / 110                128
+//   backward  fp32  155 / 73   171 / 138   177 / 171   183 / 204   191 / 229   203 / 270                160
+//   backward  bf16  128 / 48   139 / 87    140 / 108   142 / 121   145 / 144   147 / 151                224
+// They are cut until about CUT_TO workgroups are in flight, a tile each at least.  Forward + backward (us) for 512 / 768 / 1024: 2 x 32768 x 768 bf16
+// 430 / 432 / 442, 8 x 4096 x 768 bf16 250 / 224 / 225; at least 1 / 2 / 4 tiles: 1 x 10007 x 301 fp16 62 / 70 / 78, 1 x 2048 x 256 fp32 26 / 34 / 51.
+// (A single pass over the chunks, each waiting for the one before it, was no faster, 184 + 284 us for the first: what a tile waits for others costs more
 // than its second reading.)
-constexpr int CUT_BELOW = 192, CUT_TO = 768;
-static ScanPlan scan_plan(int n, int length, int width) {
+constexpr int CUT_MOST = 224, CUT_TO = 768;
+static int cut_below(int dtype, bool backward) { return dtype == LEGO_F32 ? (backward ? 160 : 96) : (backward ? CUT_MOST : 128); }
+static ScanPlan scan_plan(int n, int length, int width, int below) {
     ScanPlan p;
     p.slices = (width + SC_CH - 1) / SC_CH;
     p.tiles = (length + SC_TILE - 1) / SC_TILE;
     const int64_t wgs = (int64_t)n * p.slices;
     p.chunks = 1;
-    if (wgs < CUT_BELOW && p.tiles >= 4) {
+    if (wgs < below && p.tiles >= 4) {
         const int64_t want = (CUT_TO + wgs - 1) / wgs;
         p.chunks = (int)(want < p.tiles ? want : p.tiles);
     }
@@ -667,10 +674,10 @@ static int scan_sizes(const char* who, int dtype, int n, int length, int width) 
     return 0;
 }
 
-// floats: the partial rows of sum q, then the chunks' compositions
+// floats: the partial rows of sum q, then the chunks' compositions, of whichever call cuts
 extern "C" int64_t lego_gated_scan_workspace(int n, int length, int width) {
     if (n <= 0 || length <= 0 || width <= 0) return 0;
-    const ScanPlan p = scan_plan(n, length, width);
+    const ScanPlan p = scan_plan(n, length, width, CUT_MOST);
     return (p.chunks > 1 ? 2 * (int64_t)n * p.chunks * width : 0) + (int64_t)p.rows * p.chunks * width;
 }
 
@@ -683,7 +690,7 @@ extern "C" int lego_gated_scan_fwd(const void* x, int64_t x_sn, int64_t x_sl, co
     LEGO_REQUIRE(length > 0, "lego_gated_scan_fwd: length 0 (the state is the answer)");
     LEGO_REQUIRE(x && r && i && lam && h && last, "lego_gated_scan_fwd: NULL operand");
     if (int rc = scan_strides("lego_gated_scan_fwd", x_sl, r_sl, i_sl, 0)) return rc;
-    const ScanPlan p = scan_plan(n, length, width);
+    const ScanPlan p = scan_plan(n, length, width, cut_below(dtype, false));
     LEGO_REQUIRE(p.chunks == 1 || (workspace != nullptr && workspace_floats >= lego_gated_scan_workspace(n, length, width)),
                  "lego_gated_scan_fwd: workspace of %lld floats, lego_gated_scan_workspace says %lld", (long long)workspace_floats,
                  (long long)lego_gated_scan_workspace(n, length, width));
@@ -716,7 +723,7 @@ extern "C" int lego_gated_scan_bwd(const void* x, int64_t x_sn, int64_t x_sl, co
     if (width == 0) return 0;
     LEGO_REQUIRE(x && r && i && gh && lam && tiles && dx && dr && di && dlam, "lego_gated_scan_bwd: NULL operand");
     if (int rc = scan_strides("lego_gated_scan_bwd", x_sl, r_sl, i_sl, gh_sl)) return rc;
-    const ScanPlan p = scan_plan(n, length, width);
+    const ScanPlan p = scan_plan(n, length, width, cut_below(dtype, true));
     LEGO_REQUIRE(workspace != nullptr && workspace_floats >= lego_gated_scan_workspace(n, length, width),
                  "lego_gated_scan_bwd: workspace of %lld floats, lego_gated_scan_workspace says %lld", (long long)workspace_floats,
                  (long long)lego_gated_scan_workspace(n, length, width));

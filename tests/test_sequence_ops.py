@@ -323,7 +323,8 @@ def test_scan_and_its_gradients(shape, mask, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape,mask,dtype",
-                         [((200, 260, 24), m, t) for m in (None, "prefix", "holes") for t in TYPES] +          # a workgroup a sequence, 5 tiles each
+                         [((200, 260, 24), m, t) for m in (None, "prefix", "holes") for t in TYPES] +          # forward: a workgroup a sequence, 5 tiles each
+                         [((230, 260, 24), m, t) for m in (None, "holes") for t in TYPES] +                    # backward too
                          [((190, 1280, 24), m, torch.bfloat16) for m in (None, "prefix")] +                    # chunks of 4 tiles
                          [((52, 193, 2561), "prefix", torch.float16), ((52, 193, 2561), None, torch.float32)])    # backward: workgroups with two sequences
 def test_scan_of_many_sequences(shape, mask, dtype):
