@@ -122,8 +122,9 @@ def _mask_of(what, mask, shape, like):
         _refuse(what, f"mask has to be of shape {tuple(shape)} on {like.device}")
 
 
-def _run(function, op, operands, *rest):
+def _run(what, function, op, operands, *rest):
     """the op on its operands and the rest of its arguments: through its autograd.Function where a gradient is wanted, else below the autograd key"""
+    _ops.refuse_tangents(what, operands)
     if torch.is_grad_enabled():
         for t in operands:
             if t is not None and t.requires_grad:
@@ -153,7 +154,7 @@ def gated_scan(x, r, i, lam, mask=None, state=None, sharpness=8.0):
     if not 0 < sharpness < math.inf:
         _refuse(what, f"sharpness {sharpness} is not a positive number")
     _need_gpu(x, what)
-    h, last, _ = _run(_ops.GatedScan, _ops.scan_op, (x, r, i, lam, state), x, r, i, lam, mask, state, float(sharpness), False)
+    h, last, _ = _run(what, _ops.GatedScan, _ops.scan_op, (x, r, i, lam, state), x, r, i, lam, mask, state, float(sharpness), False)
     return h, last
 
 
@@ -173,6 +174,7 @@ def gated_scan_step(x, r, i, lam, state, mask=None, sharpness=8.0):
     if torch.is_grad_enabled() and (x.requires_grad or r.requires_grad or i.requires_grad or lam.requires_grad or state.requires_grad):
         _refuse(what, "has no gradient; use gated_scan, or call it under torch.no_grad()")
     _need_gpu(x, what)
+    _ops.refuse_tangents(what, (x, r, i, lam, state))
     with _ops.below_autograd():
         return _ops.scan_step_op(x, r, i, lam, state, mask, float(sharpness))
 
@@ -193,7 +195,7 @@ def rms_norm(x, w, eps=1e-6):
     _norm_width(what, x)
     _weights(what, x, x.shape[-1:], w)
     _need_gpu(x, what)
-    n = _run(_ops.BlockNorm, _ops.norm_op, (x, w), _rows2(x), None, None, None, None, w, float(eps), 0, False)[1]
+    n = _run(what, _ops.BlockNorm, _ops.norm_op, (x, w), _rows2(x), None, None, None, None, w, float(eps), 0, False)[1]
     return n if x.dim() == 2 else n.view(x.shape)
 
 
@@ -217,7 +219,7 @@ def gated_residual_norm(x, o, gate, post_w, scale, next_w=None, eps=1e-6, act="s
     if next_w is not None:
         _weights(what, x, x.shape[-1:], next_w)
     _need_gpu(x, what)
-    y, n, _ = _run(_ops.BlockNorm, _ops.norm_op, (x, o, gate, post_w, scale, next_w), _rows2(x), _rows2(o), _rows2(gate), post_w, scale, next_w,
+    y, n, _ = _run(what, _ops.BlockNorm, _ops.norm_op, (x, o, gate, post_w, scale, next_w), _rows2(x), _rows2(o), _rows2(gate), post_w, scale, next_w,
                    float(eps), _ops.K.GATE_ACTS[act], False)
     if x.dim() != 2:
         y, n = y.view(x.shape), n if next_w is None else n.view(x.shape)
@@ -252,7 +254,7 @@ def token_logprobs(logits, targets=None, k=0, mask=None):
         mask = mask.reshape(-1, items) if mask.dim() > 2 else mask.expand(rows.shape)
     if targets is not None and not flat:
         targets = targets.reshape(-1)
-    logp, entropy, _, top, index = _run(_ops.TokenLogprobs, _ops.logprobs_op, (logits,), rows, targets, mask, k)
+    logp, entropy, _, top, index = _run(what, _ops.TokenLogprobs, _ops.logprobs_op, (logits,), rows, targets, mask, k)
     if flat:
         return logp, entropy, top, index
     lead = logits.shape[:-1]

@@ -18,10 +18,11 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.library import custom_op, register_autograd, register_fake
 
 from . import kernels as K
-from ._lib import call
+from ._lib import LegoHipError, call
 
 NS = "lego_hip"
 
@@ -496,16 +497,41 @@ def _define(name, schema, impl, fake):
     return getattr(torch.ops.lego_hip, name).default
 
 
+def refuse_tangents(what, operands):
+    """forward-mode derivatives: a dual operand need not require a gradient, and the kernels would answer as if it had no tangent"""
+    if forward_ad._current_level >= 0:                       # (outside a dual level nothing is looked at)
+        for t in operands:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise LegoHipError(f"{what}: no forward-mode derivative; reverse mode (backward, torch.autograd.grad) differentiates it")
+
+
 def _differentiable(name, function, wants):
     """the Autograd entry of an op: `function` where one of its operands (those at the places `wants`) requires a gradient"""
     op = getattr(torch.ops.lego_hip, name).default
 
     def entry(*args):
+        refuse_tangents(name, args)
         if torch.is_grad_enabled() and any(args[q] is not None and args[q].requires_grad for q in wants):
             return function.apply(*args)
         with below_autograd():
             return op(*args)
     _LIB.impl(name, entry, "Autograd")
+
+
+def _not_differentiable(name):
+    """the Autograd entry of an op that has no gradient: its outputs say so where a backward pass reaches them"""
+    op = getattr(torch.ops.lego_hip, name).default
+
+    class NoGradient(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, *args):
+            with below_autograd():
+                return op(*args)
+
+        @staticmethod
+        def backward(ctx, *grads):
+            raise LegoHipError(f"lego_hip::{name} has no gradient")
+    _differentiable(name, NoGradient, [q for q, a in enumerate(op._schema.arguments) if "Tensor" in str(a.type)])
 
 
 def _once(what):
@@ -558,11 +584,14 @@ class GatedScan(torch.autograd.Function):
         x, r, i, lam, mask, tiles = ctx.saved_tensors
         if gh is None:
             gh = torch.zeros_like(x, memory_format=torch.contiguous_format)
-        dx, dr, di, dlam, dstate = scan_bwd_op(gh, glast, x, r, i, lam, mask, tiles, ctx.sharpness)
+        with below_autograd():
+            dx, dr, di, dlam, dstate = scan_bwd_op(gh, glast, x, r, i, lam, mask, tiles, ctx.sharpness)
         return dx, dr, di, dlam, None, dstate if ctx.has_state else None, None, None
 
 
 _differentiable("gated_scan", GatedScan, (0, 1, 2, 3, 5))
+_not_differentiable("gated_scan_bwd")
+_not_differentiable("gated_scan_step")
 
 
 # ---- block_norm: y = x + scale act(gate) rmsnorm(o) post_w, next = rmsnorm(y) next_w, over rows [rows, width] -> (y, next, the rows'
@@ -613,11 +642,13 @@ class BlockNorm(torch.autograd.Function):
             gn = torch.zeros_like(x, memory_format=torch.contiguous_format)
         if next_w is None and gy is None:
             gy = torch.zeros_like(x, memory_format=torch.contiguous_format)
-        out = norm_bwd_op(gy if o is not None else None, gn if next_w is not None else None, x, o, gate, post_w, scale, next_w, stat, ctx.eps, ctx.act)
+        with below_autograd():
+            out = norm_bwd_op(gy if o is not None else None, gn if next_w is not None else None, x, o, gate, post_w, scale, next_w, stat, ctx.eps, ctx.act)
         return tuple(None if t is None else g for g, t in zip(out, (x, o, gate, post_w, scale, next_w))) + (None, None, None)
 
 
 _differentiable("block_norm", BlockNorm, range(6))
+_not_differentiable("block_norm_bwd")
 
 
 # ---- token_logprobs: rows of logits [rows, items] -> (log probability of the target, entropy, [rows, 2] maximum and ln of the sum of
@@ -649,10 +680,12 @@ class TokenLogprobs(torch.autograd.Function):
     def backward(ctx, g_logp, g_entropy, g_stat, g_top, g_index):
         _once("lego_hip::token_logprobs")
         logits, targets, mask, stat, entropy, index = ctx.saved_tensors
-        return logprobs_bwd_op(g_logp, g_entropy, g_top, logits, targets, mask, stat, entropy, index), None, None, None
+        with below_autograd():
+            return logprobs_bwd_op(g_logp, g_entropy, g_top, logits, targets, mask, stat, entropy, index), None, None, None
 
 
 _differentiable("token_logprobs", TokenLogprobs, (0,))
+_not_differentiable("token_logprobs_bwd")
 
 
 OPS = ("gather_rows", "scatter_add_rows", "linear", "linear_bwd", "glove_project", "glove_project_bwd", "glove_project_bwd_table", "conv3_relu_mask",
