@@ -124,6 +124,8 @@ def _mask_of(what, mask, shape, like):
 
 def _run(what, function, op, operands, *rest):
     """the op on its operands and the rest of its arguments: through its autograd.Function where a gradient is wanted, else below the autograd key"""
+    if torch.compiler.is_compiling():                # traced: the registered op, whose autograd entry does the rest
+        return op(*rest)
     _ops.refuse_tangents(what, operands)
     if torch.is_grad_enabled():
         for t in operands:
@@ -174,6 +176,8 @@ def gated_scan_step(x, r, i, lam, state, mask=None, sharpness=8.0):
     if torch.is_grad_enabled() and (x.requires_grad or r.requires_grad or i.requires_grad or lam.requires_grad or state.requires_grad):
         _refuse(what, "has no gradient; use gated_scan, or call it under torch.no_grad()")
     _need_gpu(x, what)
+    if torch.compiler.is_compiling():
+        return _ops.scan_step_op(x, r, i, lam, state, mask, float(sharpness))
     _ops.refuse_tangents(what, (x, r, i, lam, state))
     with _ops.below_autograd():
         return _ops.scan_step_op(x, r, i, lam, state, mask, float(sharpness))

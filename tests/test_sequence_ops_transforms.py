@@ -1,6 +1,8 @@
-"""The sequence operators under torch's transforms: forward-mode derivatives are refused, never answered with zeros.
+"""The sequence operators under torch's transforms: forward-mode derivatives are refused, never answered with zeros, and the public functions are traced whole.
 
 Without a GPU the registered ops get a stand-in on the CPU (plain torch forms), so that the Python above the kernels is what runs."""
+from concurrent.futures import ThreadPoolExecutor
+
 import pytest
 import torch
 
@@ -30,6 +32,15 @@ def _scan_impl(x, r, i, lam, mask, state, c, keep):
     return h, last.clone(), torch.zeros(x.shape[0], -(-x.shape[1] // K.SCAN_TILE) if keep else 0, x.shape[2])
 
 
+def _with_autograd(f):
+    """a kernel is called below autograd; a stand-in that differentiates a plain form does so on a thread of its own"""
+    def g(*args):
+        with ThreadPoolExecutor(1) as pool:
+            return pool.submit(f, *args).result()
+    return g
+
+
+@_with_autograd
 def _scan_bwd_impl(gh, glast, x, r, i, lam, mask, tiles, c):
     with torch.enable_grad():
         leaves = [t.detach().requires_grad_() for t in (x, r, i, lam, torch.zeros(x.shape[0], x.shape[2]))]
@@ -43,6 +54,7 @@ def _norm_impl(x, o, gate, post_w, scale, next_w, eps, act, keep):
     return x.new_empty(0) if o is None else y, x.new_empty(0) if next_w is None else _norm(y, next_w, eps), stat
 
 
+@_with_autograd
 def _norm_bwd_impl(dy, dn, x, o, gate, post_w, scale, next_w, stat, eps, act):
     with torch.enable_grad():
         leaves = [t.detach().requires_grad_() if t is not None else None for t in (x, o, gate, post_w, scale, next_w)]
@@ -60,6 +72,7 @@ def _probs_impl(logits, targets, mask, k):
     return lp.gather(1, at)[:, 0], -(lp.exp() * lp).sum(1), torch.zeros(len(lp), 2), top, index.int()
 
 
+@_with_autograd
 def _probs_bwd_impl(gl, ge, gt, logits, targets, mask, stat, entropy, index):
     with torch.enable_grad():
         x = logits.detach().requires_grad_()
@@ -144,3 +157,46 @@ def test_forward_mode_is_refused_below_the_public_functions(on_the_cpu):
         for how in (_jvp, _dual):
             with pytest.raises(LegoHipError, match="forward-mode"):
                 how(f, v)
+
+
+def _compiled_calls(dev):
+    """name -> (a function of leaves that require a gradient, the leaves)"""
+    g = torch.Generator().manual_seed(2)
+    x, r, i = (torch.randn(2, 70, 8, generator=g).to(dev) for _ in range(3))
+    lam, st, w, s = torch.randn(8, generator=g).to(dev), torch.randn(2, 8, generator=g).to(dev), torch.ones(8, device=dev), torch.randn(8, generator=g).to(dev)
+    t = torch.tensor([1, 0], device=dev)
+    return {
+        "scan": (lambda x, r, i, lam, st: F.gated_scan(x, r, i, lam, state=st), (x, r, i, lam, st)),
+        "rms": (lambda x, w: (F.rms_norm(x, w),), (x, w)),
+        "tail": (lambda x, o, g, w, s: F.gated_residual_norm(x, o, g, w, s, w), (x, r, i, w, s)),
+        "tail alone": (lambda x, o, g, w, s: F.gated_residual_norm(x, o, g, w, s)[:1], (x, r, i, w, s)),
+        "probs": (lambda x: F.token_logprobs(x, t, k=3)[:3], (st,)),
+        "probs of a batch": (lambda x: F.token_logprobs(x, k=2)[1:3], (x,)),
+    }
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("name", list(_compiled_calls("cpu")))
+def test_public_functions_compile_whole(request, name, dev):
+    if dev == "cpu":
+        request.getfixturevalue("on_the_cpu")
+    f, leaves = _compiled_calls(dev)[name]
+    whole = torch.compile(f, fullgraph=True, backend="aot_eager")
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(whole(*leaves), f(*leaves)))
+    live = [t.clone().requires_grad_() for t in leaves]
+    want, got = f(*live), whole(*live)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    up = [torch.ones_like(t) for t in want]
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, live, up), torch.autograd.grad(want, live, up)))
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_the_single_step_compiles_whole(request, dev):
+    if dev == "cpu":
+        request.getfixturevalue("on_the_cpu")
+    x, r, i, st = (torch.randn(3, 8, generator=torch.Generator().manual_seed(q)).to(dev) for q in range(4))
+    lam = torch.randn(8, generator=torch.Generator().manual_seed(9)).to(dev)
+    f = lambda *a: F.gated_scan_step(*a)      # noqa: E731
+    whole = torch.compile(f, fullgraph=True, backend="aot_eager")
+    assert all(torch.equal(a, b) for a, b in zip(whole(x, r, i, lam, st), f(x, r, i, lam, st)))
