@@ -77,6 +77,17 @@ __device__ __forceinline__ fv sigmoid_of(fv v) {
     return s;
 }
 
+// 1 - s of s = sigmoid(v) as e^-v s: its bits are there for open gates too, where the difference has lost them.  (From v = -88 on s is 0, and so is what
+// is multiplied by this; the argument is kept below where e^-v overflows, for no 0 * inf.)  What the exponential costs, us: 64 x 2048 x 256 fp32
+// 210 -> 214, bf16 147 -> 157, 2 x 32768 x 768 bf16 217 -> 226.  The plain difference for waves in which no gate is open far enough to matter
+// in 16 bits was slower than both, 169 and 240: the branch parts loads from arithmetic.
+__device__ __forceinline__ fv rest_of(fv v, fv s) {
+    fv o;
+#pragma unroll
+    for (int j = 0; j < SC_VC; ++j) o[j] = __builtin_amdgcn_exp2f(fminf(-1.44269504088896340736f * v[j], 126.f)) * s[j];
+    return o;
+}
+
 __device__ __forceinline__ bool all_near(fv k) {
     bool near = true;
 #pragma unroll
@@ -438,8 +449,8 @@ __device__ __forceinline__ void gradients(In& in, bool some, fv k, fv (&sr)[STEP
             q_all += q;
             if (!in.whole && t + s >= left) continue;
             store_at<T, SC_VC, FULL>(d.dx + row + s * width, at_d, c, width, in.kept(s, du * si[s]));
-            store_at<T, SC_VC, FULL>(d.dr + row + s * width, at_d, c, width, in.kept(s, q * (1.f - sr[s])));
-            store_at<T, SC_VC, FULL>(d.di + row + s * width, at_d, c, width, in.kept(s, du * u * (1.f - si[s])));
+            store_at<T, SC_VC, FULL>(d.dr + row + s * width, at_d, c, width, in.kept(s, q * rest_of(in.at(0, s), sr[s])));
+            store_at<T, SC_VC, FULL>(d.di + row + s * width, at_d, c, width, in.kept(s, du * u * rest_of(in.at(3, s), si[s])));
         }
     } else {
 #pragma unroll

@@ -1,0 +1,34 @@
+"""The sequence operators at the ends of their ranges: saturated and overflowing gates, operands that a mode has no use for, very many rows, the forms that cut
+sequences and rows, against the plain 64-bit forms of test_sequence_ops.py and with its tolerances."""
+import math
+
+import pytest
+import torch
+
+from legommenders_amd import functional as F
+from tests.test_sequence_ops import SCAN_CELL, SCAN_STEP, TYPES, _lam, _memory, _rand, check, scan_64
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("side", [1, -1, 0])
+def test_gradients_of_saturated_gates(side, dtype):
+    """1 - sigmoid(v) = e^-v sigmoid(v) has its bits for large v too, where 1 minus a rounded sigmoid has lost them (0.9 % at 12, all from 17 on)"""
+    n, length, width = 2, 70, 24
+    g = torch.Generator().manual_seed(5)
+    r, i = ((8 + 17 * torch.rand(n, length, width, generator=g)) for _ in range(2))
+    if side <= 0:
+        r = torch.where(torch.rand(r.shape, generator=g) < (0.5 if side == 0 else 1.0), -r, r)
+        i = torch.where(torch.rand(i.shape, generator=g) < (0.5 if side == 0 else 1.0), -i, i)
+    x, r, i = (t.to(dtype) for t in (_rand(1, n, length, width), r, i))
+    lam, st, gh, gl = _lam(width, lo=0.9, hi=0.999), _rand(2, n, width), _rand(3, n, length, width, dtype=dtype), _rand(4, n, width)
+    want = scan_64(x, r, i, lam, None, st, 8.0, gh, gl)
+    for name, v in (("dr", r.double()), ("di", i.double())):                                 # that form's 1 - sigmoid loses bits in 64 bits as well
+        want[name] = tuple(t * torch.sigmoid(-v) / (1 - torch.sigmoid(v)) for t in want[name])
+    leaves = [t.cuda().requires_grad_() for t in (x, r, i, lam, st)]
+    h, last = F.gated_scan(*leaves[:4], state=leaves[4])
+    grads = torch.autograd.grad((h, last), leaves, (gh.cuda(), gl.cuda()))
+    many = SCAN_STEP * _memory(length) + SCAN_CELL + 2 * 25                                  # the exponentials' arguments are up to 25 in size: a rounding each
+    # closed gates: sqrt(2 k) 2^-63 for each step where sigmoid(r) would be below 2^-126 -- none here (r >= -25)
+    for got, name in zip((h, last, *grads), ("h", "last", "dx", "dr", "di", "dlam", "dstate")):
+        check(got, *want[name], 2 * many + (n * length if name == "dlam" else 0))
