@@ -13,6 +13,8 @@
 // What bounds it: in fp32 memory (64 x 2048 x 256: forward 110 us, 4.9 TB/s; backward 204 us, 4.6 TB/s); in 16 bits, with half the bytes, the vector
 // units (forward 74 us of 54 for the same cells: 50 instructions a cell, 5 of them transcendental).  Cut into chunks, 2 x 32768 x 768 bf16: forward
 // 170 us, backward 228.  512 x 50 x 256 fp32 with ragged lengths: 18 us forward, 39 backward.
+#include <float.h>
+
 #include <type_traits>
 
 #include "seq_common.hpp"
@@ -108,13 +110,16 @@ __device__ __forceinline__ fv shuffle_down(fv v, int lanes) {
     return s;
 }
 
-// -c softplus(lam) of this lane's channels
+// -c softplus(lam) of this lane's channels; finite where it overflows, so that a gate that is shut (sigmoid 0: every step that is not live) decays by 1
 template <bool FULL>
 __device__ __forceinline__ fv rates(const float* __restrict__ lam, float sharpness, int c, int width) {
     const fv v = load<float, SC_VC, FULL>(lam, c, width);
     fv k;
 #pragma unroll
-    for (int j = 0; j < SC_VC; ++j) k[j] = c + j < width ? -sharpness * softplus(v[j]) : 0.f;
+    for (int j = 0; j < SC_VC; ++j) {
+        const float q = -sharpness * softplus(v[j]);
+        k[j] = c + j < width ? (q < -FLT_MAX ? -FLT_MAX : q) : 0.f;    // (NaN stays NaN)
+    }
     return k;
 }
 
@@ -442,10 +447,11 @@ __device__ __forceinline__ void gradients(In& in, bool some, fv k, fv (&sr)[STEP
         for (int s = STEPS - 1; s >= 0; --s) {
             const fv G = in.at(1, s) + back, xs = in.at(2, s), du = G * beta[s], u = si[s] * xs, l = k * sr[s];
             back = a[s] * G;
-            fv lb;                                                         // l / beta tends to 0 with l (as -sqrt(-l / 2)): where beta has become 0, so has l
+            // l / beta tends to 0 with l (as -sqrt(-l / 2)): where beta has become 0, so has l.  l comes last: it may be as large as fp32 goes, where back is 0
+            fv rb;
 #pragma unroll
-            for (int q = 0; q < SC_VC; ++q) lb[q] = beta[s][q] > 0.f ? l[q] * __builtin_amdgcn_rcpf(beta[s][q]) : 0.f;
-            const fv q = in.kept(s, back * (before[s] * l - u * a[s] * lb));
+            for (int q = 0; q < SC_VC; ++q) rb[q] = beta[s][q] > 0.f ? __builtin_amdgcn_rcpf(beta[s][q]) : 0.f;
+            const fv q = in.kept(s, back * (before[s] - u * a[s] * rb) * l);
             q_all += q;
             if (!in.whole && t + s >= left) continue;
             store_at<T, SC_VC, FULL>(d.dx + row + s * width, at_d, c, width, in.kept(s, du * si[s]));

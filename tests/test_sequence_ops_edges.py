@@ -32,3 +32,24 @@ def test_gradients_of_saturated_gates(side, dtype):
     # closed gates: sqrt(2 k) 2^-63 for each step where sigmoid(r) would be below 2^-126 -- none here (r >= -25)
     for got, name in zip((h, last, *grads), ("h", "last", "dx", "dr", "di", "dlam", "dstate")):
         check(got, *want[name], 2 * many + (n * length if name == "dlam" else 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["lam", "sharpness"])
+@pytest.mark.parametrize("length", [5, 64, 300])
+def test_decays_that_overflow(kind, length):
+    """a rate beyond fp32 (lam infinite, or a huge sharpness): a live step forgets the state, a masked one and the places behind the sequence keep it"""
+    n, width = 3, 24
+    x, r, i, st, gh, gl = _rand(1, n, length, width), _rand(2, n, length, width), _rand(3, n, length, width), 1e3 * _rand(4, n, width), _rand(5, n, length, width), _rand(6, n, width)
+    m = torch.rand(n, length, generator=torch.Generator().manual_seed(7)) < 0.5
+    m[1] = False
+    lam = _lam(width)
+    lam[::3] = math.inf if kind == "lam" else 3.0                                            # 3e38 softplus(3) is beyond fp32, 3e38 softplus(the others) is not
+    far = torch.where(torch.isinf(lam), 1e4, lam)                                            # there a is 0 in 64 bits too, and every term is finite
+    want = scan_64(x, r, i, far, m, st, 8.0, gh, gl) if kind == "lam" else scan_64(x, r, i, torch.full((width,), 1e4), m, st, 8.0, gh, gl)
+    leaves = [t.cuda().requires_grad_() for t in (x, r, i, lam, st)]
+    h, last = F.gated_scan(*leaves[:4], mask=m.cuda(), state=leaves[4], sharpness=8.0 if kind == "lam" else 3e38)
+    grads = torch.autograd.grad((h, last), leaves, (gh.cuda(), gl.cuda()))
+    many = SCAN_STEP * _memory(length) + SCAN_CELL
+    for got, name in zip((h, last, *grads), ("h", "last", "dx", "dr", "di", "dlam", "dstate")):
+        check(got, *want[name], 2 * many + (n * length if name == "dlam" else 0))
