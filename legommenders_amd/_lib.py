@@ -113,9 +113,17 @@ class LegoHipError(RuntimeError):
     pass
 
 
-def build(verbose: bool = False) -> str:
-    """Compile every HIP source for gfx950 into legommenders_amd/csrc/liblego_hip.so (in-tree)."""
-    cmd = ["make", "-C", CSRC, "-j4"]
+def _up_to_date() -> bool:
+    """the library is there and younger than all it is built from (the objects need not be there: a copy of the tree may come without them)"""
+    sources = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hip", ".hpp")) or f == "Makefile"] + [HEADER]
+    return os.path.exists(LIB_PATH) and os.path.getmtime(LIB_PATH) >= max(os.path.getmtime(f) for f in sources)
+
+
+def build(verbose: bool = False, force: bool = False) -> str:
+    """Compile every HIP source for gfx950 into legommenders_amd/csrc/liblego_hip.so (in-tree); without `force` only what is older than its sources."""
+    if not force and _up_to_date():
+        return LIB_PATH
+    cmd = ["make", "-C", CSRC, "-j4"] + ["-B"] * force
     res = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or res.returncode != 0:
         print(res.stdout[-4000:])
