@@ -444,7 +444,8 @@ int lego_gated_scan_step(const void* x, int64_t x_sn, const void* r, int64_t r_s
  * y and next are contiguous; stat [halves, rows] keeps 1 / rms(o) (where there is an o), then 1 / rms(y) (where there is a next_w), for _bwd
  * (NULL = not wanted).
  * _bwd: dy (may be NULL where next_w is given) and dn are the gradients of y and next; dx, dout (of o), dgate contiguous; dpost_w, dscale,
- * dnext_w [width] are written, not added to, in a fixed order of summation. */
+ * dnext_w [width] are written, not added to, in a fixed order of summation.  Operands without a use -- gate with act 0, or gate, post_w and scale
+ * without o -- are not read, and their gradients are not written. */
 #define LEGO_BLOCK_NORM_MAX_WIDTH 16384
 int64_t lego_block_norm_workspace(int rows, int width);                          /* floats, for _bwd */
 int lego_block_norm_fwd(const void* x, int64_t ldx, const void* o /*nullable*/, int64_t ldo, const void* gate, int64_t ldg, int dtype, int act,

@@ -437,10 +437,12 @@ def block_norm_bwd(dy, dn, x, o, gate, post_w, scale, next_w, eps, act, stat):
     _agree("block_norm_bwd", x, (o, gate, dy, dn), ((post_w, (width,)), (scale, (width,)), (next_w, (width,)),
                                                     (stat, ((o is not None) + (next_w is not None), rows))))
     stat = stat.contiguous()
-    new = lambda t: None if t is None else torch.empty(rows, width, dtype=x.dtype, device=x.device)      # noqa: E731
-    dx, do, dgate = new(x), new(o), new(gate)
-    make = torch.zeros if rows == 0 else torch.empty
-    dpw, dsc, dnw = (None if t is None else make(width, dtype=torch.float32, device=x.device) for t in (post_w, scale, next_w))
+    # (what the kernels do not use -- a gate without an activation, the block's operands without a block -- they write no gradient of)
+    make = lambda t, written, *shape: None if t is None else (torch.empty if written and rows else torch.zeros)(      # noqa: E731
+        *shape, dtype=x.dtype if len(shape) == 2 else torch.float32, device=x.device)
+    block = o is not None
+    dx, do, dgate = (make(t, written, rows, width) for t, written in ((x, True), (o, True), (gate, block and act != 0)))
+    dpw, dsc, dnw = (make(t, written, width) for t, written in ((post_w, block), (scale, block), (next_w, True)))
     if rows == 0:
         return dx, do, dgate, dpw, dsc, dnw
     x, o, gate, dy, dn = (_last_dense(t) for t in (x, o, gate, dy, dn))

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from legommenders_amd import functional as F
+from legommenders_amd import kernels as K
 from tests.test_sequence_ops import SCAN_CELL, SCAN_STEP, TYPES, _lam, _memory, _rand, check, scan_64
 
 
@@ -53,3 +54,48 @@ def test_decays_that_overflow(kind, length):
     many = SCAN_STEP * _memory(length) + SCAN_CELL
     for got, name in zip((h, last, *grads), ("h", "last", "dx", "dr", "di", "dlam", "dstate")):
         check(got, *want[name], 2 * many + (n * length if name == "dlam" else 0))
+
+
+@pytest.fixture
+def filled():
+    """fresh memory is full of NaN"""
+    torch.use_deterministic_algorithms(True)
+    yield
+    torch.use_deterministic_algorithms(False)
+
+
+UNUSED = [dict(o=1, post_w=1, scale=1, next_w=1, gate=1), dict(o=1, post_w=1, scale=1, gate=1), dict(next_w=1, gate=1), dict(next_w=1, post_w=1), dict(next_w=1, scale=1)]
+
+
+@pytest.mark.parametrize("given", UNUSED)
+def test_nothing_uninitialised_comes_back_for_what_a_norm_does_not_use(given, filled, monkeypatch):
+    """the kernels write no gradient of a gate without an activation, or of a block's operands without a block: the registered op's are zeros"""
+    wrote = []
+    monkeypatch.setattr(K, "_agree", lambda *a, **k: None)
+    monkeypatch.setattr(K, "_launch", lambda t, name, *a: wrote.append(name))
+    x, w = torch.ones(3, 8), torch.ones(8)
+    o, gate = (x if given.get(k) else None for k in ("o", "gate"))
+    pw, sc, nw = (w if given.get(k) else None for k in ("post_w", "scale", "next_w"))
+    out = K.block_norm_bwd(x, x if nw is not None else None, x, o, gate, pw, sc, nw, 1e-6, 0, torch.ones(2, 3))
+    assert wrote == ["lego_block_norm_bwd"]
+    for name, t in zip(("gate", "post_w", "scale"), (out[2], out[3], out[4])):
+        used = name != "gate" and o is not None
+        assert t is None or used or bool((t == 0).all()), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("given", UNUSED)
+def test_operands_that_a_norm_does_not_use(given, filled):
+    block_norm = torch.ops.lego_hip.block_norm
+    names = ("o", "gate", "post_w", "scale", "next_w")
+    x = _rand(1, 5, 12).cuda().requires_grad_()
+    ops = [None if not given.get(k) else _rand(2 + q, *((5, 12) if q < 2 else (12,))).cuda().requires_grad_() for q, k in enumerate(names)]
+    used = [t if given.get("o") or k == "next_w" else None for k, t in zip(names, ops)]
+    used[1] = None
+    grads = []
+    for a in (ops, used):
+        out = [t for t in block_norm(x, *a, 1e-6, 0, True)[:2] if t.numel()]
+        there = [x] + [t for t in ops if t is not None]
+        grads.append(torch.autograd.grad(out, there, [torch.ones_like(t) for t in out], allow_unused=True))
+    for got, want in zip(*grads):
+        assert torch.equal(got, torch.zeros_like(got) if want is None else want)
