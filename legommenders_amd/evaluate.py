@@ -17,7 +17,7 @@ import numpy as np
 import torch
 
 from . import metrics as M
-from ._lib import call
+from ._lib import LegoHipError, call
 from .engine import NamlEngine, NrmsEngine, _ptr, _stream
 
 
@@ -41,14 +41,20 @@ def gather_shards(local: torch.Tensor, n: int, process_group, world: int) -> tor
 def next_items(user_repr, item_repr, users, targets=None, k=10, seen=None, page=512):
     """What the users would click next, over the whole catalogue: scores <user, item> of every item, their softmax.
 
-    users [n] rows of user_repr; targets [n] items (optional; -1: none); seen (user_hist [n_users, S], user_hist_len [n_users]): clicks that are
-    left out of the catalogue (a target is always in).  -> dict of logp [n] of the targets, entropy [n], top [n, k] log probabilities and
+    users [n] rows of user_repr; targets [n] items (optional; outside the catalogue, as -1: none); seen (user_hist [n_users, S], user_hist_len
+    [n_users]): clicks that are left out of the catalogue (a target is always in).  -> dict of logp [n] of the targets, entropy [n], top [n, k] log probabilities and
     items [n, k] int32 (-1 where nothing is left), `page` users at a time (their scores are [page, n_items] fp32)."""
     from . import functional as F
     dev, n_items = item_repr.device, item_repr.shape[0]
-    users = torch.as_tensor(users).to(dev, torch.int64)
+    users = torch.as_tensor(users).to(torch.int64)
+    if users.dim() != 1 or users.numel() and not 0 <= int(users.min()) <= int(users.max()) < user_repr.shape[0]:
+        raise LegoHipError(f"next_items: users are rows of user_repr, 0 to {user_repr.shape[0] - 1}, in one dimension")
+    users = users.to(dev)
     if targets is not None:
         targets = torch.as_tensor(targets).to(dev, torch.int64)
+        if targets.shape != users.shape:
+            raise LegoHipError(f"next_items: targets are one item a user: {tuple(targets.shape)} for {tuple(users.shape)} users")
+        targets = torch.where((targets >= 0) & (targets < n_items), targets, -1)
     padded = torch.nn.functional.pad(item_repr, (0, 0, 0, -n_items % 4))                     # (the products' rows are multiples of 4 elements)
     out = []
     for s in range(0, users.numel(), page):
@@ -59,7 +65,8 @@ def next_items(user_repr, item_repr, users, targets=None, k=10, seen=None, page=
             hist, length = seen[0][u].long(), seen[1][u]
             S = hist.shape[1]
             mask = torch.ones(u.numel(), n_items + 1, dtype=torch.bool, device=dev)          # the last column takes the pads
-            mask.scatter_(1, torch.where(torch.arange(S, device=dev)[None] < length[:, None], hist, n_items), False)
+            there = (torch.arange(S, device=dev)[None] < length[:, None]) & (hist >= 0) & (hist < n_items)
+            mask.scatter_(1, torch.where(there, hist, n_items), False)
             if t is not None:
                 mask.scatter_(1, torch.where(t >= 0, t, n_items)[:, None], True)
             mask = mask[:, :n_items]
