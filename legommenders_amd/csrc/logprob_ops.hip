@@ -15,6 +15,8 @@
 // statistics and keys.
 #include <float.h>
 
+#include <algorithm>
+
 #include "seq_common.hpp"
 
 namespace lego {
@@ -230,6 +232,10 @@ __device__ __forceinline__ int64_t wanted(const Wanted& w, int64_t row) {
     return w.p == nullptr ? -1 : w.wide ? ((const int64_t*)w.p)[row] : ((const int32_t*)w.p)[row];
 }
 
+static Wanted wanted_from(const void* targets, int wide, int64_t row) {
+    return {targets == nullptr ? nullptr : wide ? (const void*)((const int64_t*)targets + row) : (const void*)((const int32_t*)targets + row), wide};
+}
+
 struct Outputs { float *logp, *entropy, *stat, *top; int32_t* index; };
 
 // the wanted item's logit, -inf where a mask hides it (asked for before the row is read: its latency is then hidden)
@@ -443,6 +449,10 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(const T* __restrict__
 
 struct LogprobPlan { int chunks, per, threads; };
 
+// A launch has fewer than 2^32 lanes: more rows than that go in several, one after the other (forward, only rows that are one chunk: fewer than 512 rows
+// are cut, into 512 workgroups and some)
+static int rows_a_launch(const LogprobPlan& p) { return (int)(((1ll << 32) - 1) / p.threads / p.chunks); }
+
 // Forward: a workgroup a row, of 1024 lanes where a row has 8192 vectors (of 16 bytes) and more, else of 256 (2048 x 30522 bf16: 33 us with 256 lanes, 50
 // with 1024, whose ends are too much of so short a row; 512 x 65238 fp32, 50 alternatives: 47 and 37 us).  Fewer than 512 rows do not fill
 // the 256 CUs: they are cut into chunks of at least 2048 vectors until there are about 512 workgroups, and joined by a second launch.
@@ -462,6 +472,7 @@ static LogprobPlan bwd_plan(int items, int dtype) {
     const int vec = dtype == LEGO_F32 ? 4 : 8;
     const int64_t vectors = ((int64_t)items + 2 * vec - 2) / vec;
     LogprobPlan p;
+    p.threads = 256;
     p.per = 2048;
     p.chunks = (int)((vectors + p.per - 1) / p.per);
     return p;
@@ -495,19 +506,22 @@ extern "C" int lego_token_logprobs_fwd(const void* logits, int64_t ld, int dtype
     LEGO_REQUIRE(p.chunks == 1 || (workspace != nullptr && workspace_words >= lego_token_logprobs_workspace(rows, items, dtype, k)),
                  "lego_token_logprobs_fwd: workspace of %lld words, lego_token_logprobs_workspace says %lld", (long long)workspace_words,
                  (long long)lego_token_logprobs_workspace(rows, items, dtype, k));
-    LEGO_REQUIRE((int64_t)rows * p.chunks < (1ll << 31), "lego_token_logprobs_fwd: %d rows in %d chunks", rows, p.chunks);
-    const Wanted w{targets, targets_64};
-    const Outputs out{logp, entropy, stat, top, index};
     float4* stats = (float4*)workspace;
     u64* keys = (u64*)workspace + 2 * (int64_t)rows * p.chunks;
-    const dim3 grid((unsigned)((int64_t)rows * p.chunks));
-#define GO(MASK, NT) hipLaunchKernelGGL((logprobs_fwd_kernel<T, MASK, NT>), grid, dim3(NT), 0, ST, (const T*)logits, ld, mask, mask_ld, w, out, stats, keys, items, k, \
-                                        p.chunks, p.per)
-#define JOIN(NT) hipLaunchKernelGGL((logprobs_join_kernel<T, NT>), dim3(rows), dim3(NT), 0, ST, (const T*)logits, ld, mask, mask_ld, w, out, stats, keys, items, k, p.chunks)
+    const int most = rows_a_launch(p);
+#define GO(MASK, NT) hipLaunchKernelGGL((logprobs_fwd_kernel<T, MASK, NT>), grid, dim3(NT), 0, ST, x, ld, m, mask_ld, w, out, stats, keys, items, k, p.chunks, p.per)
+#define JOIN(NT) hipLaunchKernelGGL((logprobs_join_kernel<T, NT>), dim3(rows), dim3(NT), 0, ST, x, ld, m, mask_ld, w, out, stats, keys, items, k, p.chunks)
     LEGO_BY_TYPE(dtype, {
-        if (p.threads == 1024) { if (mask != nullptr) GO(true, 1024); else GO(false, 1024); }
-        else if (mask != nullptr) GO(true, 256); else GO(false, 256);
-        if (p.chunks > 1) { if ((int64_t)p.chunks * k > 256) JOIN(1024); else JOIN(256); }
+        for (int64_t r = 0; r < rows; r += most) {
+            const dim3 grid((unsigned)(std::min<int64_t>(most, rows - r) * p.chunks));
+            const T* x = (const T*)logits + r * ld;
+            const uint8_t* m = mask != nullptr ? mask + r * mask_ld : nullptr;
+            const Wanted w = wanted_from(targets, targets_64, r);
+            const Outputs out{logp + r, entropy + r, stat + 2 * r, top != nullptr ? top + r * k : nullptr, index != nullptr ? index + r * k : nullptr};
+            if (p.threads == 1024) { if (mask != nullptr) GO(true, 1024); else GO(false, 1024); }
+            else if (mask != nullptr) GO(true, 256); else GO(false, 256);
+            if (p.chunks > 1) { if ((int64_t)p.chunks * k > 256) JOIN(1024); else JOIN(256); }
+        }
     });
 #undef GO
 #undef JOIN
@@ -521,13 +535,19 @@ extern "C" int lego_token_logprobs_bwd(const void* logits, int64_t ld, int dtype
     if (rows == 0) return 0;
     LEGO_REQUIRE(logits && stat && entropy && dlogits && (g_top == nullptr || (k > 0 && index)), "lego_token_logprobs_bwd: NULL operand");
     const LogprobPlan p = bwd_plan(items, dtype);
-    LEGO_REQUIRE((int64_t)rows * p.chunks < (1ll << 31), "lego_token_logprobs_bwd: %d rows in %d chunks", rows, p.chunks);
-    const Wanted w{targets, targets_64};
-    const Grads g{g_logp, g_entropy, g_top};
-    const dim3 grid((unsigned)((int64_t)rows * p.chunks));
-#define GO(MASK) hipLaunchKernelGGL((logprobs_bwd_kernel<T, MASK>), grid, dim3(256), 0, ST, (const T*)logits, ld, mask, mask_ld, w, stat, entropy, index, g, \
-                                    (T*)dlogits, items, k, p.chunks, p.per)
-    LEGO_BY_TYPE(dtype, { if (mask != nullptr) GO(true); else GO(false); });
+    const int most = rows_a_launch(p);
+#define GO(MASK) hipLaunchKernelGGL((logprobs_bwd_kernel<T, MASK>), grid, dim3(256), 0, ST, (const T*)logits + r * ld, ld, m, mask_ld, w, stat + 2 * r, entropy + r, \
+                                    i, g, (T*)dlogits + r * items, items, k, p.chunks, p.per)
+    LEGO_BY_TYPE(dtype, {
+        for (int64_t r = 0; r < rows; r += most) {
+            const dim3 grid((unsigned)(std::min<int64_t>(most, rows - r) * p.chunks));
+            const uint8_t* m = mask != nullptr ? mask + r * mask_ld : nullptr;
+            const Wanted w = wanted_from(targets, targets_64, r);
+            const Grads g{g_logp != nullptr ? g_logp + r : nullptr, g_entropy != nullptr ? g_entropy + r : nullptr, g_top != nullptr ? g_top + r * k : nullptr};
+            const int32_t* i = index != nullptr ? index + r * k : nullptr;
+            if (mask != nullptr) GO(true); else GO(false);
+        }
+    });
 #undef GO
     return check_launch("lego_token_logprobs_bwd");
 }

@@ -88,10 +88,10 @@ __device__ __forceinline__ vec<T, N> load_some(const T* __restrict__ row, int c,
 
 }  // namespace lego
 
-// one instantiation of BODY for the activations' type, named T there
-#define LEGO_BY_TYPE(dtype, BODY)                                                                                                                  \
-    do {                                                                                                                                           \
-        if ((dtype) == LEGO_F32) { using T = float; BODY; }                                                                                        \
-        else if ((dtype) == LEGO_BF16) { using T = __bf16; BODY; }                                                                                 \
-        else { using T = _Float16; BODY; }                                                                                                         \
+// one instantiation of the statements behind `dtype` for the activations' type, named T there
+#define LEGO_BY_TYPE(dtype, ...)                                                                                                                       \
+    do {                                                                                                                                               \
+        if ((dtype) == LEGO_F32) { using T = float; __VA_ARGS__; }                                                                                     \
+        else if ((dtype) == LEGO_BF16) { using T = __bf16; __VA_ARGS__; }                                                                              \
+        else { using T = _Float16; __VA_ARGS__; }                                                                                                      \
     } while (0)

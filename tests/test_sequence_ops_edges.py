@@ -7,7 +7,7 @@ import torch
 
 from legommenders_amd import functional as F
 from legommenders_amd import kernels as K
-from tests.test_sequence_ops import SCAN_CELL, SCAN_STEP, TYPES, _lam, _memory, _rand, check, scan_64
+from tests.test_sequence_ops import SCAN_CELL, SCAN_STEP, TYPES, _lam, _memory, _rand, check, logprobs_64, scan_64
 
 
 @pytest.mark.gpu
@@ -99,3 +99,27 @@ def test_operands_that_a_norm_does_not_use(given, filled):
         grads.append(torch.autograd.grad(out, there, [torch.ones_like(t) for t in out], allow_unused=True))
     for got, want in zip(*grads):
         assert torch.equal(got, torch.zeros_like(got) if want is None else want)
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_launch_has_workgroups():
+    """2^24 rows of a workgroup of 256 lanes each are 2^32 lanes, one more than a launch takes"""
+    rows, items, k = (1 << 24) + 5, 3, 2
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(rows, items, generator=g, device="cuda").half().requires_grad_()
+    t = torch.randint(-1, items, (rows,), generator=g, device="cuda").int()
+    m = torch.rand(rows, items, generator=g, device="cuda") < 0.9
+    m[:, 1] = True
+    logp, entropy, top, index = F.token_logprobs(x, t, k=k, mask=m)
+    gl, ge, gt = torch.randn(rows, generator=g, device="cuda"), torch.randn(rows, generator=g, device="cuda"), torch.randn(rows, k, generator=g, device="cuda")
+    dx, = torch.autograd.grad((logp, entropy, top), x, (gl, ge, gt))
+    for a in range(0, rows, 1 << 22):                                                        # each row against a call of its own part, and both sides of the border
+        s = slice(a, min(a + (1 << 22), rows))
+        p = x.detach()[s].requires_grad_()
+        part = F.token_logprobs(p, t[s], k=k, mask=m[s])
+        assert all(torch.equal(u[s], v) for u, v in zip((logp, entropy, top, index), part))
+        assert torch.equal(dx[s], torch.autograd.grad(part[:3], p, (gl[s], ge[s], gt[s]))[0])
+    w = logprobs_64(x.detach()[-7:].cpu(), t[-7:].cpu().long(), k, m[-7:].cpu())
+    for got, name in ((logp, "logp"), (entropy, "entropy"), (top, "top")):
+        check(got[-7:], w[name], 20.0, 100)
+    assert torch.equal(index[-7:].cpu().long(), w["index"])
