@@ -38,7 +38,7 @@ import os
 os.environ.setdefault("GPU_MAX_HW_QUEUES", "8")      # before HIP initialises: see legommenders_amd/__init__.py
 
 import argparse
-import gc
+import contextlib
 import json
 import os
 import sys
@@ -314,6 +314,7 @@ def main():
     _lib.lib()                                     # fail loudly if the HIP extension is missing
     from legommenders_amd.synthetic import MIND_SMALL, glove_like, init_naml_params, init_nrms_params, make_world
     from legommenders_amd.train_step import DeviceData, TrainStep
+    from legommenders_amd.trainer import frozen_heap
 
     cfg = dict(MIND_SMALL)
     if args.small:
@@ -335,6 +336,8 @@ def main():
             torch.distributed.barrier()
         torch.cuda.synchronize()
 
+    heap = contextlib.ExitStack()                  # the interpreter's full collections leave out what is there by now, as while the trainer trains
+    heap.enter_context(frozen_heap())
     ts = make_ts(args.model, data, force=args.force_dist, embed=args.embed)
     # Device wake-up before the W warm-up steps: half a second of a dummy product.  The driver's command (`--steps 20 --warmup 5`) reaches
     # the timed region 3 ms after the first launch of a process that has spent seconds building tables on the host; on a fresh box that
@@ -373,10 +376,6 @@ def main():
     in_region = {"naml": {"conv3_fwd", "gather_rows_in_step", "expand_rows_in_step"}, "nrms": {"qkv_fwd_item"}}[args.model]
     # every bracketed step costs ~0.08 ms of event / barrier-packet overhead (tools/step_profile.py): short runs bracket two steps
     every = args.time_every if args.steps > 40 or args.time_every == 0 else max(args.time_every, args.steps // 2)
-    # Whether the interpreter's next full collection (36 ms over the 170 000 objects that the imports leave) falls into the timed region depends on how many
-    # objects the imports made: a few more modules, or byte code that is already compiled, moved it from the imports into the 200 steps (0.549 -> 0.60 to
-    # 0.69 ms a step, the host behind the device).  freeze() takes no time and leaves the collector on: what exists now is not looked through again.
-    gc.freeze()
     dt, timers, loss = timed_steps(ts, args.steps, args.warmup, barrier, every, tags=in_region)
     host_ms = timed_steps.host_s / args.steps * 1e3
     if dist_on:
