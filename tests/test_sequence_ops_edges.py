@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from legommenders_amd import functional as F
+from legommenders_amd import _lib, functional as F
 from legommenders_amd import kernels as K
 from tests.test_sequence_ops import SCAN_CELL, SCAN_STEP, TYPES, _lam, _memory, _rand, check, logprobs_64, scan_64
 
@@ -123,3 +123,131 @@ def test_more_rows_than_a_launch_has_workgroups():
     for got, name in ((logp, "logp"), (entropy, "entropy"), (top, "top")):
         check(got[-7:], w[name], 20.0, 100)
     assert torch.equal(index[-7:].cpu().long(), w["index"])
+
+
+class _Bands:
+    """tensors inside larger buffers: what surrounds an input is NaN (all bits set, where whole numbers are), what surrounds an output has to stay"""
+
+    def __init__(self, guard=256):
+        self.guard, self.outs = guard, []
+
+    def input(self, t):
+        t = t.contiguous()
+        fill = math.nan if t.dtype.is_floating_point else (255 if t.dtype == torch.uint8 else -1)
+        buf = torch.full((t.numel() + 2 * self.guard,), fill, dtype=t.dtype, device="cuda")
+        inside = buf[self.guard:self.guard + t.numel()].view(t.shape)
+        inside.copy_(t)
+        return inside
+
+    def output(self, *shape, dtype=torch.float32):
+        count = math.prod(shape)
+        buf = torch.full((count + 2 * self.guard,), 7, dtype=dtype, device="cuda")
+        self.outs.append(buf)
+        return buf[self.guard:self.guard + count].view(shape)
+
+    def check(self):
+        torch.cuda.synchronize()
+        assert all(bool((b[:self.guard] == 7).all()) and bool((b[-self.guard:] == 7).all()) for b in self.outs)
+
+
+DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,masked", [((1, 1030, 33), False), ((1, 10007, 301), False), ((2, 4096, 64), True), ((3, 705, 1), True), ((190, 1280, 24), False), ((52, 193, 2561), True)])
+def test_cut_scans_stay_inside_their_buffers(shape, masked, dtype):
+    n, length, width = shape
+    b, p, st = _Bands(), K._ptr, K._stream()
+    x, r, i, gh = (b.input(_rand(q, n, length, width, dtype=dtype)) for q in range(4))
+    lam, state, glast = b.input(_lam(width)), b.input(_rand(5, n, width)), b.input(_rand(6, n, width))
+    m = None
+    if masked:
+        m = (torch.rand(n, length, generator=torch.Generator().manual_seed(1)) < 0.7).to(torch.uint8)
+        m[0, : length // 2] = 0
+        m = b.input(m)
+    want = F.gated_scan(*(t.clone() for t in (x, r, i, lam)), mask=None if m is None else m.clone(), state=state.clone())
+    h, last, tiles = b.output(n, length, width, dtype=dtype), b.output(n, width), b.output(n, -(-length // 64), width)
+    size = _lib.lib().lego_gated_scan_workspace(n, length, width)
+    ws = b.output(size)
+    s, ms = (length * width, width), 0 if m is None else length
+    _lib.call("lego_gated_scan_fwd", p(x), *s, p(r), *s, p(i), *s, DT[dtype], p(lam), 8.0, p(m), ms, p(state), p(h), p(last), p(tiles), p(ws), size, n, length, width, st)
+    assert torch.equal(h, want[0]) and torch.equal(last, want[1])
+    d = [b.output(n, length, width, dtype=dtype) for _ in range(3)] + [b.output(width), b.output(n, width)]
+    ws.fill_(math.nan)                                                                       # (nothing in it is taken over)
+    _lib.call("lego_gated_scan_bwd", p(x), *s, p(r), *s, p(i), *s, p(gh), *s, DT[dtype], p(lam), 8.0, p(m), ms, p(tiles.clone()), p(glast), *(p(t) for t in d), p(ws), size,
+              n, length, width, st)
+    leaves = [t.clone().requires_grad_() for t in (x, r, i, lam, state)]
+    out = F.gated_scan(*leaves[:4], mask=None if m is None else m.clone(), state=leaves[4])
+    for got, g in zip(d, torch.autograd.grad(out, leaves, (gh.clone(), glast.clone()))):
+        assert torch.equal(got, g) and bool(torch.isfinite(got).all())
+    b.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,k,masked", [((1, 400001), 20, False), ((1, 400001), 128, True), ((5, 65238), 50, True), ((3, 131075), 0, False), ((300, 16411), 7, True), ((600, 65239), 10, False)])
+def test_cut_rows_stay_inside_their_buffers(shape, k, masked, dtype):
+    rows, items = shape
+    b, p, st = _Bands(), K._ptr, K._stream()
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = b.input(torch.randn(rows, items, generator=g, device="cuda").to(dtype))
+    t = b.input(torch.randint(-1, items, (rows,), generator=g, device="cuda"))
+    m = b.input((torch.rand(rows, items, generator=g, device="cuda") < 0.7).to(torch.uint8)) if masked else None
+    gl, ge, gt = (b.input(torch.randn(*s, generator=g, device="cuda")) for s in ((rows,), (rows,), (rows, k)))
+    leaf = x.clone().requires_grad_()
+    want = F.token_logprobs(leaf, t.clone(), k=k, mask=None if m is None else m.clone())
+    logp, entropy, stat, top, index = b.output(rows), b.output(rows), b.output(rows, 2), b.output(rows, k), b.output(rows, k, dtype=torch.int32)
+    size = _lib.lib().lego_token_logprobs_workspace(rows, items, DT[dtype], k)
+    ws = b.output(max(size, 2), dtype=torch.int64)
+    ms = 0 if m is None else items
+    _lib.call("lego_token_logprobs_fwd", p(x), items, DT[dtype], p(m), ms, p(t), 1, k, p(logp), p(entropy), p(stat), p(top), p(index), p(ws), size, rows, items, st)
+    assert all(torch.equal(u, v) for u, v in zip((logp, entropy, top, index), want))
+    assert not bool(torch.isnan(logp).any()) and bool(torch.isfinite(entropy).all())             # (a masked target's logp is -inf)
+    d = b.output(rows, items, dtype=dtype)
+    _lib.call("lego_token_logprobs_bwd", p(x), items, DT[dtype], p(m), ms, p(t), 1, k, p(stat), p(entropy), p(index), p(gl), p(ge), p(gt) if k else None, p(d), rows, items, st)
+    assert torch.equal(d, torch.autograd.grad(want[:3] if k else want[:2], leaf, (gl, ge, gt)[:3 if k else 2])[0]) and bool(torch.isfinite(d).all())
+    b.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width", [(9, 1), (130, 33), (2049, 257), (7, 1025), (5, 2051), (5, 4099), (3, 5120), (3, 8193), (2, 16384), (600, 4100)])
+def test_norms_stay_inside_their_buffers(rows, width, dtype):
+    b, p, st = _Bands(), K._ptr, K._stream()
+    x, o, g, gy, gn = (b.input(_rand(q, rows, width, dtype=dtype)) for q in range(5))
+    pw, sc, nw = (b.input(_rand(5 + q, width)) for q in range(3))
+    leaves = [t.clone().requires_grad_() for t in (x, o, g, pw, sc, nw)]
+    want = F.gated_residual_norm(*leaves, act="silu")
+    y, n, stat = b.output(rows, width, dtype=dtype), b.output(rows, width, dtype=dtype), b.output(2, rows)
+    _lib.call("lego_block_norm_fwd", p(x), width, p(o), width, p(g), width, DT[dtype], 2, p(pw), p(sc), p(nw), 1e-6, p(y), p(n), p(stat), rows, width, st)
+    assert torch.equal(y, want[0]) and torch.equal(n, want[1])
+    d = [b.output(rows, width, dtype=dtype) for _ in range(3)] + [b.output(width) for _ in range(3)]
+    size = _lib.lib().lego_block_norm_workspace(rows, width)
+    ws = b.output(size)
+    _lib.call("lego_block_norm_bwd", p(x), width, p(o), width, p(g), width, DT[dtype], 2, p(pw), p(sc), p(nw), 1e-6, p(gy), width, p(gn), width, p(stat), *(p(t) for t in d),
+              p(ws), size, rows, width, st)
+    for got, w in zip(d, torch.autograd.grad(want, leaves, (gy.clone(), gn.clone()))):
+        assert torch.equal(got, w) and bool(torch.isfinite(got).all())
+    b.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,items", [(520, 65536), (513, 70001)])
+@pytest.mark.parametrize("kind", ["plain", "rounded", "constant", "lowest", "two"])
+def test_the_largest_of_uncut_rows_of_1024_lanes(kind, rows, items, dtype):
+    """k up to 16 (64 groups of lanes) and above (256), rows in which more elements are equal than the list of candidates holds"""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(rows, items, generator=g, device="cuda")
+    x = dict(plain=x, rounded=x.round(), constant=torch.full_like(x, -0.5), lowest=torch.where(x > 3, x, torch.finfo(dtype).min), two=(x > 0).float())[kind].to(dtype)
+    order = torch.sort(x.float(), dim=1, descending=True, stable=True)
+    lp = torch.log_softmax(x.double(), 1)
+    for k in (1, 10, 16, 17, 65, 128):
+        logp, entropy, top, index = F.token_logprobs(x, order.indices[:, 0], k=k)
+        assert torch.equal(index.long(), order.indices[:, :k])
+        want = lp.gather(1, order.indices[:, :k]).cpu()
+        finite = x.double().masked_fill(x == torch.finfo(dtype).min, 0).abs().amax(1).cpu() + 12.0
+        some = want > -1e30                                                                  # (behind a row's large elements come the lowest ones)
+        check(torch.where(some.cuda(), top, 0.0), torch.where(some, want, 0.0), finite[:, None], items / 256 + 40)
+        check(logp, lp.gather(1, order.indices[:, :1])[:, 0].cpu(), finite, items / 256 + 40)
