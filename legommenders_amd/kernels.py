@@ -424,6 +424,8 @@ def block_norm_fwd(x, o, gate, post_w, scale, next_w, eps, act, keep=False):
     y = torch.empty(rows, width, dtype=x.dtype, device=dev) if o is not None else None
     nxt = torch.empty(rows, width, dtype=x.dtype, device=dev) if next_w is not None else None
     stat = torch.empty((o is not None) + (next_w is not None), rows if keep else 0, dtype=torch.float32, device=dev)
+    if rows == 0 and stat.shape[0]:                              # (the C entry tells a block by its pointer: that of no rows is NULL)
+        return y, nxt, stat
     x, o, gate = _last_dense(x), _last_dense(o), _last_dense(gate)
     post_w, scale, next_w = (None if t is None else t.contiguous() for t in (post_w, scale, next_w))
     _launch(x, "lego_block_norm_fwd", _at(x), _ld(x), _at(o), _ld(o), _at(gate), _ld(gate), _DTYPES[x.dtype], act, _at(post_w), _at(scale),

@@ -251,3 +251,17 @@ def test_the_largest_of_uncut_rows_of_1024_lanes(kind, rows, items, dtype):
         some = want > -1e30                                                                  # (behind a row's large elements come the lowest ones)
         check(torch.where(some.cuda(), top, 0.0), torch.where(some, want, 0.0), finite[:, None], items / 256 + 40)
         check(logp, lp.gather(1, order.indices[:, :1])[:, 0].cpu(), finite, items / 256 + 40)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(0, 8), (2, 0, 8), (0, 3, 5)])
+@pytest.mark.parametrize("next_norm", [False, True])
+@pytest.mark.parametrize("grad", [False, True])
+def test_tails_of_no_rows(shape, next_norm, grad):
+    x, o, g = (torch.zeros(shape, device="cuda", requires_grad=grad) for _ in range(3))
+    w = torch.ones(shape[-1], device="cuda", requires_grad=grad)
+    y, n = F.gated_residual_norm(x, o, g, w, w, w if next_norm else None)
+    assert y.shape == shape and (n.shape == shape if next_norm else n is None)
+    if grad:
+        dx, dw = torch.autograd.grad(y.sum() + (n.sum() if next_norm else 0), (x, w))
+        assert dx.shape == shape and bool((dw == 0).all())
