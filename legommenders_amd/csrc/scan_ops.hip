@@ -36,12 +36,13 @@ using fv = vec<float, SC_VC>;
 struct Seq { const void* p; int64_t sn, sl; };                     // [n, length, width] with its strides; channels are contiguous
 
 // softplus to about 1e-7 relative on the hardware exponential and logarithm: ln(1 + t) = ln(u) t / (u - 1) with u = 1 + t rounded takes the
-// rounding of u back out; e^v = 2^hi (1 + lo ln 2) keeps the part of v log2(e) that one fp32 number drops
+// rounding of u back out; e^v = 2^hi (1 + lo ln 2) keeps the part of v log2(e) that one fp32 number drops.  Below -104 it is 0 in fp32 (for v = -inf the
+// two parts would be inf - inf)
 __device__ __forceinline__ float softplus(float v) {
     const float hi = v * 1.44269504088896340736f, lo = __builtin_fmaf(v, 1.44269504088896340736f, -hi) + v * 1.92596299112661746887e-8f;
     const float e = __builtin_amdgcn_exp2f(hi), t = __builtin_fmaf(e, lo * 0.69314718055994530942f, e), u = 1.f + t, d = u - 1.f;
     const float s = d > 0.f ? 0.69314718055994530942f * __builtin_amdgcn_logf(u) * (t * __builtin_amdgcn_rcpf(d)) : t;
-    return v > 20.f ? v : s;
+    return v > 20.f ? v : v < -104.f ? 0.f : s;
 }
 
 // l = k sigmoid(r) <= 0, a = e^l, beta = sqrt(1 - a^2) = sqrt((1 - a)(1 + a)), 2 channels.  1 - a would cancel near 1: for l >= -0.5

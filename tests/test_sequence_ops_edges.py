@@ -265,3 +265,25 @@ def test_tails_of_no_rows(shape, next_norm, grad):
     if grad:
         dx, dw = torch.autograd.grad(y.sum() + (n.sum() if next_norm else 0), (x, w))
         assert dx.shape == shape and bool((dw == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("length", [1, 70, 300])
+def test_decays_of_one(length):
+    """softplus(-inf) is 0: the channel keeps its state for ever, takes nothing in, and has no gradient but the state's"""
+    n, width = 2, 24
+    x, r, i, st, gh, gl = _rand(1, n, length, width), _rand(2, n, length, width), _rand(3, n, length, width), _rand(4, n, width), _rand(5, n, length, width), _rand(6, n, width)
+    lam = _lam(width)
+    lam[::4] = -math.inf
+    want = scan_64(x, r, i, lam, None, st, 8.0, gh, gl)
+    dlam, terms = want["dlam"]                                                               # (that form's sigmoid / softplus is 0 / 0 there)
+    want["dlam"] = tuple(torch.where(torch.isinf(lam), 0.0, t) for t in (dlam, terms))
+    leaves = [t.cuda().requires_grad_() for t in (x, r, i, lam, st)]
+    h, last = F.gated_scan(*leaves[:4], state=leaves[4])
+    grads = torch.autograd.grad((h, last), leaves, (gh.cuda(), gl.cuda()))
+    many = SCAN_STEP * _memory(length) + SCAN_CELL
+    for got, name in zip((h, last, *grads), ("h", "last", "dx", "dr", "di", "dlam", "dstate")):
+        check(got, *want[name], 2 * many + (n * length if name == "dlam" else 0))
+    assert torch.equal(last.cpu()[:, ::4], st[:, ::4])
+    h1, new = F.gated_scan_step(*(t.detach()[:, 0] for t in leaves[:3]), leaves[3].detach(), leaves[4].detach())
+    assert torch.equal(new.cpu()[:, ::4], st[:, ::4]) and bool(torch.isfinite(new).all())
