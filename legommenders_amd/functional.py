@@ -10,7 +10,6 @@ ROCm implementations only, and CPU tensors raise `LegoHipError` here before they
 from __future__ import annotations
 
 import itertools
-import math
 
 import torch
 
@@ -95,6 +94,7 @@ def dot_ce(user, items):
 # ------------------------------------------------------------------------------------------ sequence operators
 # fp32, bf16 or fp16 activations (kept), fp32 weights and states; strided rows are taken as they are.  A step that a mask (0 / False) hides is
 # never used, whatever it holds.  (The checks run on every call of operators that take microseconds: they build no message unless they refuse.)
+_LEAST, _MOST = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
 _TYPES = frozenset((torch.float32, torch.bfloat16, torch.float16))
 
 
@@ -153,8 +153,8 @@ def gated_scan(x, r, i, lam, mask=None, state=None, sharpness=8.0):
         _weights(what, x, (n, width), state)
     if mask is not None:
         _mask_of(what, mask, (n, length), x)
-    if not 0 < sharpness < math.inf:
-        _refuse(what, f"sharpness {sharpness} is not a positive number")
+    if not _LEAST <= sharpness <= _MOST:
+        _refuse(what, f"sharpness {sharpness} is not a positive number of fp32")
     _need_gpu(x, what)
     h, last, _ = _run(what, _ops.GatedScan, _ops.scan_op, (x, r, i, lam, state), x, r, i, lam, mask, state, float(sharpness), False)
     return h, last
@@ -171,8 +171,8 @@ def gated_scan_step(x, r, i, lam, state, mask=None, sharpness=8.0):
     _weights(what, x, x.shape, state)
     if mask is not None:
         _mask_of(what, mask, x.shape[:1], x)
-    if not 0 < sharpness < math.inf:
-        _refuse(what, f"sharpness {sharpness} is not a positive number")
+    if not _LEAST <= sharpness <= _MOST:
+        _refuse(what, f"sharpness {sharpness} is not a positive number of fp32")
     if torch.is_grad_enabled() and (x.requires_grad or r.requires_grad or i.requires_grad or lam.requires_grad or state.requires_grad):
         _refuse(what, "has no gradient; use gated_scan, or call it under torch.no_grad()")
     _need_gpu(x, what)

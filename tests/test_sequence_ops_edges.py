@@ -7,6 +7,7 @@ import torch
 
 from legommenders_amd import _lib, functional as F
 from legommenders_amd import kernels as K
+from legommenders_amd._lib import LegoHipError
 from tests.test_sequence_ops import SCAN_CELL, SCAN_STEP, TYPES, _lam, _memory, _rand, check, logprobs_64, scan_64
 
 
@@ -287,3 +288,13 @@ def test_decays_of_one(length):
     assert torch.equal(last.cpu()[:, ::4], st[:, ::4])
     h1, new = F.gated_scan_step(*(t.detach()[:, 0] for t in leaves[:3]), leaves[3].detach(), leaves[4].detach())
     assert torch.equal(new.cpu()[:, ::4], st[:, ::4]) and bool(torch.isfinite(new).all())
+
+
+@pytest.mark.parametrize("sharpness", [1e39, 1e300, 1e-300, math.inf, math.nan, 0.0, -8.0])
+def test_a_sharpness_that_fp32_does_not_hold_is_refused(sharpness):
+    """the kernels take it in 32 bits: beyond them it would be infinite there, and 0 below"""
+    x, lam, st = torch.zeros(2, 5, 8), torch.zeros(8), torch.zeros(2, 8)
+    with pytest.raises(LegoHipError, match="sharpness"):
+        F.gated_scan(x, x, x, lam, sharpness=sharpness)
+    with pytest.raises(LegoHipError, match="sharpness"):
+        F.gated_scan_step(st, st, st, lam, st, sharpness=sharpness)
