@@ -6,7 +6,14 @@
 // in one pass: x, o and gate are read once, y and n written once.  Without a block (o = NULL) y = x and only n is written.  HBM-bound: a row
 // lives in the registers of 1 to 16 waves (16- / 8-byte loads, 4 channels a lane), the weights of a lane's channels stay in registers over the rows
 // of a persistent workgroup, and the next row's loads are in flight while a row is summed -- without that the two dependent sums of a row left the
-// memory idle (65536 x 1024 bf16, backward: 454 us, 222 with it; 4.8 TB/s, as a copy of that size).
+// memory idle (65536 x 1024 bf16, backward: 454 us, 212 with it; 5.1 TB/s, as a copy of that size).
+//
+// That holds for widths of 256 to 4096 that 4 divides.  Others are right, and slower than memory (32 M channels, fp32, TB/s of
+// what a pass has to move; forward / backward of both halves, at 1024 5.5 / 5.0):
+//   narrow rows leave lanes of their one wave idle                                            32: 2.6 / 1.7     64: 4.3 / 3.0
+//   widths that 4 does not divide load single elements, in the widest form of their waves    257: 2.9 / 2.2   1001: 4.3 / 4.3   1025: 4.3 / 3.9
+//   above 4096 a row takes 1024 lanes, which have 128 registers each: two rows spill        5120: 5.1 / 1.8   8192: 5.2 / 2.4  16384: 2.2 / 1.2
+//   both                                                                                    4099: 0.7 / 0.3   8193: 1.1 / 0.5
 //
 // Backward, with d = dy + rms_y^-1 (dn next_w - yh mean(dn next_w yh)) the gradient of y:  dx = d,  e = d scale act post_w,
 //   do = rms_o^-1 (e - oh mean(e oh)),  dgate = d scale oh post_w act'(gate),

@@ -10,9 +10,10 @@
 // HBM-bound: the rest is to keep the selection off that one read.  A key orders an element by (value, lower index first) and is unique; while it
 // reads, a lane keeps its largest key only.  The k-th largest of 64 (k <= 16) or 256 groups of lanes' keys is a lower bound of the k-th largest
 // element, so only the few lanes at or above it can own one of the k: the workgroup reads those lanes' vectors again (about k lanes' shares of
-// the row, from the caches), collects what reaches the bound and ranks it by counting.  If more than the list holds reach it (lanes that own
-// very many large elements), the k are taken one at a time instead.  Few rows are cut into chunks, and a second launch joins the chunks'
-// statistics and keys.
+// the row, from the caches), collects what reaches the bound and ranks it by counting.  If more than the list holds reach it, the k are taken one
+// at a time instead, a reading of the row each.  That takes lanes that own very many large elements, or ties: in a row of equal elements all that the first
+// k - 1 groups' lanes own come before the k-th group's first (512 x 65536, 1024 lanes: from k = 10 in bf16 -- 150 us there, 1690 for k = 128, against 20
+// and 30 of ordinary rows --, from k = 65 in fp32).  Few rows are cut into chunks, and a second launch joins the chunks' statistics and keys.
 #include <float.h>
 
 #include <algorithm>
@@ -454,7 +455,8 @@ struct LogprobPlan { int chunks, per, threads; };
 static int rows_a_launch(const LogprobPlan& p) { return (int)(((1ll << 32) - 1) / p.threads / p.chunks); }
 
 // Forward: a workgroup a row, of 1024 lanes where a row has 8192 vectors (of 16 bytes) and more, else of 256 (2048 x 30522 bf16: 33 us with 256 lanes, 50
-// with 1024, whose ends are too much of so short a row; 512 x 65238 fp32, 50 alternatives: 47 and 37 us).  Fewer than 512 rows do not fill
+// with 1024, whose ends are too much of so short a row, one call after another; 45 with 256 behind a backward pass, which leaves none of the logits in the
+// cache; 512 x 65238 fp32, 50 alternatives: 47 and 37 us).  Fewer than 512 rows do not fill
 // the 256 CUs: they are cut into chunks of at least 2048 vectors until there are about 512 workgroups, and joined by a second launch.
 static LogprobPlan fwd_plan(int rows, int items, int dtype) {
     const int vec = dtype == LEGO_F32 ? 4 : 8;

@@ -10,9 +10,10 @@
 // The backward pass keeps no h: the forward pass saves the fp32 state at the head of every tile (1/64 of the cells), the tile's states are
 // formed again from it in fp32, and G_t = dh_t + a_(t+1) G_(t+1) is the same composition from the other end.
 //
-// What bounds it: in fp32 memory (64 x 2048 x 256: forward 110 us, 4.9 TB/s; backward 204 us, 4.6 TB/s); in 16 bits, with half the bytes, the vector
-// units (forward 74 us of 54 for the same cells: 50 instructions a cell, 5 of them transcendental).  Cut into chunks, 2 x 32768 x 768 bf16: forward
-// 170 us, backward 228.  512 x 50 x 256 fp32 with ragged lengths: 18 us forward, 39 backward.
+// What bounds it: in fp32 memory (64 x 2048 x 256: forward 114 us, 4.7 TB/s; backward 214 us, 4.4 TB/s); in 16 bits, with half the bytes, the vector
+// units (the same cells: forward 65 us, backward 155; a copy of their bytes 54 and 94; forward 50 instructions a cell, 5 of them transcendental, backward two more
+// of those).  Cut into chunks, 2 x 32768 x 768 bf16: forward 160 us, backward 225 (one call after another; 180 and 252 after other work has taken the
+// cache).  512 x 50 x 256 fp32 with ragged lengths, a tile a workgroup, most of whose waves have no live step: 17 us forward of 12, 38 backward of 24.
 #include <float.h>
 
 #include <type_traits>
@@ -27,6 +28,7 @@ template <int WAVES_, int STEPS_> struct Shape {
     static constexpr int WAVES = WAVES_, STEPS = STEPS_, RUNS = SC_GROUPS * WAVES, THREADS = 64 * WAVES;
     static_assert(STEPS * RUNS == SC_TILE && SC_VC == 2, "a tile is RUNS runs of STEPS steps");
 };
+// (This and what follows was compared before rest_of's exponential, which adds 2 to 7 % to every backward form alike; scan_plan's table is with it.)
 // Measured (us): forward 8 x 4 / 4 x 8, 64 x 2048 x 256 fp32 115 / 117, 1 x 10007 x 301 fp16 42 / 48; backward, which has the registers of 16 cells a
 // lane only in workgroups of 4 waves, 512 x 50 x 256 fp32 84 / 54, 64 x 2048 x 256 fp32 231 / 211.
 using Fwd = Shape<8, 4>;
@@ -646,14 +648,14 @@ struct ScanPlan { int slices, tiles, chunks, per, rows; };
 // A workgroup a (sequence, 64 channels) reads every input once, and from some number of them on is as fast as memory or the vector units allow; fewer
 // leave the GPU idle, and sequences of 4 tiles and more are then cut into chunks, which read their inputs twice.  n x 2048 x 256, us uncut / cut:
 //   workgroups        64         128         160         192         224         256
-//   forward   fp32   72 / 49    78 / 95     84 / 120    90 / 146   100 / 177   112 / 194      cut below  96
-//   forward   bf16   63 / 37    64 / 63     66 / 76     66 / 84     66 / 103    68 / 110                128
-//   backward  fp32  155 / 73   171 / 138   177 / 171   183 / 204   191 / 229   203 / 270                160
-//   backward  bf16  128 / 48   139 / 87    140 / 108   142 / 121   145 / 144   147 / 151                224
+//   forward   fp32   71 / 47    76 / 94     82 / 120    88 / 143    97 / 176   108 / 188      cut below  96
+//   forward   bf16   61 / 36    63 / 62     64 / 76     64 / 82     65 / 101    65 / 107                128
+//   backward  fp32  156 / 70   172 / 135   178 / 168   184 / 192   193 / 232   205 / 255                160
+//   backward  bf16  135 / 49   146 / 91    147 / 113   149 / 124   152 / 151   153 / 158                224
 // They are cut until about CUT_TO workgroups are in flight, a tile each at least.  Forward + backward (us) for 512 / 768 / 1024: 2 x 32768 x 768 bf16
 // 430 / 432 / 442, 8 x 4096 x 768 bf16 250 / 224 / 225; at least 1 / 2 / 4 tiles: 1 x 10007 x 301 fp16 62 / 70 / 78, 1 x 2048 x 256 fp32 26 / 34 / 51.
-// (A single pass over the chunks, each waiting for the one before it, was no faster, 184 + 284 us for the first: what a tile waits for others costs more
-// than its second reading.)
+// (A single pass over the chunks, each waiting for the one before it, was no faster: 184 us forward and 284 backward at 2 x 32768 x 768, 181 and 250 in two
+// passes at the time.  What a tile waits for others costs more than its second reading.)
 constexpr int CUT_MOST = 224, CUT_TO = 768;
 static int cut_below(int dtype, bool backward) { return dtype == LEGO_F32 ? (backward ? 160 : 96) : (backward ? CUT_MOST : 128); }
 static ScanPlan scan_plan(int n, int length, int width, int below) {

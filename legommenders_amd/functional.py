@@ -275,7 +275,8 @@ def catalogue_scores(user, items):
 def next_item_loss(user, items, targets, mask=None):
     """-mean log probability of each user's next item over a whole catalogue: user [B, D] x items [N, D] -> scalar; targets [B] (outside
     [0, N): the row does not count).  The full-softmax sibling of `dot_ce`'s sampled one: the scores are one product, their softmax and its
-    gradient one pass each."""
+    gradient one pass each.  Where 4 does not divide N, the items and the scores' gradient are copied once more into padded ones (512 users x 65 238
+    items: 5 % of the step)."""
     if targets.dim() != 1 or user.dim() != 2 or targets.shape[0] != user.shape[0]:
         _refuse("next_item_loss", f"targets are one item a user: {tuple(targets.shape)} for users {tuple(user.shape)}")
     _need_gpu(user, "next_item_loss")
