@@ -48,6 +48,9 @@ def frozen_heap():
     """While steps run, the interpreter's full collections leave out what existed before them: the 170 000 objects that the imports make cost 36 ms each
     time, and where one falls into a run of steps the host drops behind the device (200 steps then took 0.60 to 0.69 ms each; with none in them 0.549 to
     0.551, frozen or not, three runs each).  The collector stays on for what the steps make."""
+    if gc.get_freeze_count():                                      # the caller's own: left as it is
+        yield
+        return
     gc.collect()
     gc.freeze()
     try:

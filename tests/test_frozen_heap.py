@@ -29,6 +29,17 @@ def test_training_leaves_what_was_there_out_of_collections():
     assert gc.get_freeze_count() == 0                                                        # and gives it back, however it ends
 
 
+def test_a_heap_that_the_caller_froze_stays_frozen():
+    gc.freeze()
+    try:
+        n = gc.get_freeze_count()
+        with trainer.frozen_heap():
+            pass
+        assert gc.get_freeze_count() >= n - 1000                                             # (objects that went by reference count are no longer in it)
+    finally:
+        gc.unfreeze()
+
+
 def test_the_benchmark_times_the_same():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     names = {n.id for n in ast.walk(ast.parse(open(os.path.join(root, "bench.py")).read())) if isinstance(n, ast.Name)}
