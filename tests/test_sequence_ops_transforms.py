@@ -200,3 +200,12 @@ def test_the_single_step_compiles_whole(request, dev):
     f = lambda *a: F.gated_scan_step(*a)      # noqa: E731
     whole = torch.compile(f, fullgraph=True, backend="aot_eager")
     assert all(torch.equal(a, b) for a, b in zip(whole(x, r, i, lam, st), f(x, r, i, lam, st)))
+
+
+def test_ops_without_a_gradient_say_so_in_the_backward_pass(on_the_cpu):
+    st, lam = torch.randn(2, 8), torch.randn(8)
+    h, new = L.gated_scan_step(st, st, st, lam.requires_grad_(), st, None, 8.0)
+    with pytest.raises(LegoHipError, match="gated_scan_step has no gradient"):
+        h.sum().backward()
+    with torch.no_grad():
+        assert not L.gated_scan_step(st, st, st, lam, st, None, 8.0)[0].requires_grad
